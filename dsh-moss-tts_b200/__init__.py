@@ -54,6 +54,8 @@ EXPORTS = [
     "mossgpu_codec_open", "mossgpu_codec_close", "mossgpu_codec_reset", "mossgpu_codec_decode_chunk",
     "mossgpu_codec_decode_batch", "mossgpu_codec_decode_batch_device", "mossgpu_codec_decode",
     "mossgpu_codec_profile", "mossgpu_codec_profile_read", "mossgpu_codec_kernel_name", "mossgpu_codec_status",
+    "mossgpu_rope_steps", "mossgpu_rope_rotate", "mossgpu_kv8_append", "mossgpu_kv8_read",
+    "mossgpu_attention_kv8_workspace_bytes", "mossgpu_attention_kv8", "mossgpu_token_logprobs",
 ]
 
 
@@ -73,6 +75,70 @@ class SampleParams(C.Structure):
         return cls(int(greedy), temperature, top_k, top_p, repetition_penalty, int(end_greedy), min_frames,
                    greedy_frames)
 
+
+class Rope(C.Structure):
+    """mossgpu_rope.  Pointers here and below are device addresses as integers (torch's data_ptr())."""
+    _fields_ = [("steps", C.c_void_p), ("rotary_dim", C.c_int), ("interleaved", C.c_int), ("magnitude", C.c_float)]
+
+
+class RopeScaling(C.Structure):
+    """mossgpu_rope_scaling."""
+    _fields_ = [("kind", C.c_int), ("factor", C.c_double), ("original_len", C.c_double), ("slow", C.c_double),
+                ("fast", C.c_double)]
+
+
+class RopeArgs(C.Structure):
+    """mossgpu_rope_args."""
+    _fields_ = [("x", C.c_void_p), ("out", C.c_void_p), ("pos", C.c_void_p), ("x_row_stride", C.c_int64),
+                ("x_head_stride", C.c_int64), ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64),
+                ("rows", C.c_int), ("heads", C.c_int), ("head_dim", C.c_int), ("type", C.c_int), ("inverse", C.c_int)]
+
+
+class KV8Cache(C.Structure):
+    """mossgpu_kv8_cache."""
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("page_table", C.c_void_p), ("n_pages", C.c_int),
+                ("n_slots", C.c_int), ("pages_per_slot", C.c_int), ("kv_heads", C.c_int), ("head_dim", C.c_int),
+                ("format", C.c_int)]
+
+
+class SeqBatch(C.Structure):
+    """mossgpu_seq_batch."""
+    _fields_ = [("row_start", C.c_void_p), ("slot", C.c_void_p), ("ctx_len", C.c_void_p), ("n_seqs", C.c_int),
+                ("rows", C.c_int)]
+
+
+class KV8AppendArgs(C.Structure):
+    """mossgpu_kv8_append_args."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("q", C.c_void_p), ("q_out", C.c_void_p), ("pos", C.c_void_p),
+                ("k_row_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_row_stride", C.c_int64),
+                ("v_head_stride", C.c_int64), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("q_out_row_stride", C.c_int64), ("q_out_head_stride", C.c_int64), ("q_heads", C.c_int),
+                ("type", C.c_int)]
+
+
+class KV8ReadArgs(C.Structure):
+    """mossgpu_kv8_read_args."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_row_stride", C.c_int64), ("k_head_stride", C.c_int64),
+                ("v_row_stride", C.c_int64), ("v_head_stride", C.c_int64), ("type", C.c_int)]
+
+
+class AttentionKV8Args(C.Structure):
+    """mossgpu_attention_kv8_args."""
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("mask", C.c_void_p), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_size_t), ("q_row_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("out_row_stride", C.c_int64), ("out_head_stride", C.c_int64), ("q_heads", C.c_int), ("type", C.c_int),
+                ("mask_words", C.c_int), ("scale", C.c_float)]
+
+
+class LogprobArgs(C.Structure):
+    """mossgpu_logprob_args."""
+    _fields_ = [("logits", C.c_void_p), ("tokens", C.c_void_p), ("logprob", C.c_void_p), ("entropy", C.c_void_p),
+                ("top_ids", C.c_void_p), ("top_logprobs", C.c_void_p), ("row_stride", C.c_int64), ("rows", C.c_int),
+                ("vocab", C.c_int), ("type", C.c_int), ("top_k", C.c_int), ("temperature", C.c_float)]
+
+
+F32, F16, BF16 = 0, 1, 2  # element types of activations (MOSSGPU_F32 ...)
+KV_INT8, KV_E4M3 = 0, 1   # formats of the 8-bit cache (MOSSGPU_KV_INT8 ...)
 
 _f32 = np.ctypeslib.ndpointer(np.float32, flags="C_CONTIGUOUS")
 _i32 = np.ctypeslib.ndpointer(np.int32, flags="C_CONTIGUOUS")
@@ -171,8 +237,28 @@ def lib() -> C.CDLL:
         L.mossgpu_codec_kernel_name.restype = C.c_char_p
         L.mossgpu_codec_kernel_name.argtypes = [C.c_int]
         L.mossgpu_codec_status.argtypes = [C.c_void_p, C.POINTER(C.c_int)]
+        L.mossgpu_rope_steps.argtypes = [C.c_int, C.c_double, C.POINTER(RopeScaling), C.c_void_p, C.POINTER(C.c_float)]
+        L.mossgpu_rope_rotate.argtypes = [C.POINTER(Rope), C.POINTER(RopeArgs), C.c_void_p]
+        L.mossgpu_kv8_append.argtypes = [C.POINTER(KV8Cache), C.POINTER(SeqBatch), C.POINTER(Rope),
+                                         C.POINTER(KV8AppendArgs), C.c_void_p]
+        L.mossgpu_kv8_read.argtypes = [C.POINTER(KV8Cache), C.POINTER(SeqBatch), C.POINTER(KV8ReadArgs), C.c_void_p]
+        L.mossgpu_attention_kv8_workspace_bytes.restype = C.c_size_t
+        L.mossgpu_attention_kv8_workspace_bytes.argtypes = [C.POINTER(KV8Cache), C.c_int, C.c_int]
+        L.mossgpu_attention_kv8.argtypes = [C.POINTER(KV8Cache), C.POINTER(SeqBatch), C.POINTER(AttentionKV8Args),
+                                            C.c_void_p]
+        L.mossgpu_token_logprobs.argtypes = [C.POINTER(LogprobArgs), C.c_void_p]
         _LIB = L
         return L
+
+
+def rope_steps(rotary_dim: int, base: float = 10000.0, scaling: RopeScaling | None = None) -> tuple[np.ndarray, float]:
+    """(steps [rotary_dim / 2] uint64, magnitude) for a Rope: copy the steps to the device (mossgpu_rope_steps)."""
+    steps = np.zeros(max(1, rotary_dim // 2), np.uint64)
+    mag = C.c_float(1.0)
+    L = lib()
+    if L.mossgpu_rope_steps(rotary_dim, base, scaling, _ptr(steps), C.byref(mag)) != 0:
+        raise MossGpuError(L.mossgpu_op_last_error().decode(errors="replace"))
+    return steps, float(mag.value)
 
 
 def _ptr(a):

@@ -9,10 +9,13 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstdarg>
+#include <cstdio>
 #include <mutex>
 #include <string>
 
 #include "kernels.cuh"
+#include "op_support.h"
 
 namespace {
 
@@ -109,6 +112,33 @@ Layout layout_for(int R, size_t bytes) {
 }
 
 }  // namespace
+
+namespace mossgpu {
+
+int op_errorf(const char *fmt, ...) noexcept {
+    char text[256];
+    va_list ap;
+    va_start(ap, fmt);
+    std::vsnprintf(text, sizeof(text), fmt, ap);
+    va_end(ap);
+    try {
+        g_op_error = text;
+    } catch (...) {  // out of host memory: the status alone reports the failure
+    }
+    return 1;
+}
+
+int op_device(int *dev, int **status, const char *who) noexcept {
+    try {
+        if (device_setup(dev, who) != 0) return 1;
+        *status = g_status_ptr[*dev];
+        return 0;
+    } catch (...) {
+        return op_errorf("%s: out of host memory", who);
+    }
+}
+
+}  // namespace mossgpu
 
 extern "C" {
 

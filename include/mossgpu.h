@@ -263,6 +263,169 @@ int mossgpu_attention_decode_paged_noalloc(const float *q, const void *kv_layer,
                                            int pages_per_stream, const int32_t *row_slot, const int32_t *row_pos,
                                            int R, float *out, void *cuda_stream);
 
+/* ---- rotary positions, an 8-bit paged cache, attention over it, token log-probabilities ----
+ *
+ * Standalone ops in the manner of mossgpu_attention_decode_paged: DEVICE pointers unless a
+ * comment says host, no engine handle, the call only enqueues work on cuda_stream (a
+ * cudaStream_t; NULL = legacy default stream) of the calling thread's current device, on which
+ * all pointers must be usable, and may be captured into a CUDA graph.  The descriptors are host
+ * structs, read before the call returns.  Errors: non-zero return, message from
+ * mossgpu_op_last_error() (per thread); a refused call enqueues nothing.  Values that only the
+ * device sees (row bounds, slots, positions, page ids, tokens) are checked there: what is out of
+ * range is skipped and recorded for mossgpu_op_device_status: 9 = a slot or position outside the
+ * page table, 10 = a page id outside the pool, 11 = a token id >= vocab.
+ *
+ * Element types of activations: */
+enum { MOSSGPU_F32 = 0, MOSSGPU_F16 = 1, MOSSGPU_BF16 = 2 };
+
+/* Strides count elements; the innermost dimension is contiguous.  Where the base pointers and
+ * strides of a tensor are multiples of 16 bytes it moves 16 bytes at a time, otherwise element
+ * by element. */
+
+/* Rotary positions.  Pair i < rotary_dim / 2 of a head turns by pos * f_i:
+ *   y_a = magnitude (x_a cos - x_b sin),  y_b = magnitude (x_b cos + x_a sin)
+ * with (a, b) = (2i, 2i + 1) when interleaved, (i, i + rotary_dim / 2) otherwise; elements from
+ * rotary_dim on are copied.  The angle is held in whole 2^-64 turns: `steps` is
+ * round(f_i / (2 pi) 2^64) modulo 2^64, so that pos * steps, taken modulo 2^64, is the reduced
+ * angle at any position, without the loss that a product of floats has at far ones. */
+typedef struct {
+    const uint64_t *steps;  /* [rotary_dim / 2], see mossgpu_rope_steps */
+    int rotary_dim;         /* even, 2 .. head_dim */
+    int interleaved;
+    float magnitude;        /* on cos and sin; 1 unless the scaling asks for another */
+} mossgpu_rope;
+
+/* Host helper: the steps of base^(-2i / rotary_dim), scaled for contexts `factor` times longer:
+ *   0 none; 1 linear: f / factor; 2 base: base * factor^(rotary_dim / (rotary_dim - 2));
+ *   3 ramp: f where a pair makes at least `fast` turns over original_len positions, f / factor
+ *     where it makes at most `slow`, in proportion to the turns between.
+ * *magnitude (may be NULL) = 0.1 ln(factor) + 1 for the ramp, which is what it is used with as a
+ * rule, else 1.
+ * Writes `steps` (HOST memory, rotary_dim / 2 entries).  scaling NULL = none. */
+typedef struct {
+    int kind;
+    double factor;
+    double original_len;
+    double slow, fast;
+} mossgpu_rope_scaling;
+int mossgpu_rope_steps(int rotary_dim, double base, const mossgpu_rope_scaling *scaling, uint64_t *steps,
+                       float *magnitude);
+
+/* out = x rotated (or turned back, which is also the gradient of the rotation): x, out
+ * [rows][heads][head_dim], head_dim a multiple of 8 up to 256.  out may be x itself with the same
+ * strides, or must not overlap it. */
+typedef struct {
+    const void *x;
+    void *out;
+    const int32_t *pos;     /* [rows], any sign */
+    int64_t x_row_stride, x_head_stride, out_row_stride, out_head_stride;
+    int rows, heads, head_dim;
+    int type;               /* of x and out */
+    int inverse;
+} mossgpu_rope_args;
+int mossgpu_rope_rotate(const mossgpu_rope *rope, const mossgpu_rope_args *args, void *cuda_stream);
+
+/* A paged cache of 8-bit codes, the fp16 cache's layout with one byte an element and one fp32
+ * scale per (position, head) for K and one for V: value = code * scale.
+ *   int8: scale = absmax / 127, code = round-half-even(x / scale)
+ *   e4m3: scale = absmax / 448, code = the nearest e4m3 value to x / scale
+ * A head whose scale would be below 2^-126 is stored as zeros with scale 0; one that holds an
+ * infinity or a NaN as zero codes with a NaN scale, so that it reads back as NaN.  The e4m3 NaN
+ * codes (0x7f, 0xff) never occur, and attention gives no meaning to them. */
+enum { MOSSGPU_KV_INT8 = 0, MOSSGPU_KV_E4M3 = 1 };
+typedef struct {
+    void *codes;                /* [n_pages][2 (k, v)][kv_heads][16][head_dim] bytes, 16-byte aligned */
+    float *scales;              /* [n_pages][2 (k, v)][kv_heads][16], 16-byte aligned */
+    const int32_t *page_table;  /* [n_slots][pages_per_slot]; entries past a slot's length are not read */
+    int n_pages, n_slots, pages_per_slot;
+    int kv_heads, head_dim;     /* head_dim 64 or 128 */
+    int format;
+} mossgpu_kv8_cache;
+
+/* A ragged batch: sequence s owns rows row_start[s] .. row_start[s + 1] - 1 of the row tensors
+ * (row_start ascends; a sequence may own none), lives in slot[s] and has ctx_len[s] positions in
+ * the cache already: its i-th row is position ctx_len[s] + i.  The slots of a call are distinct.
+ * Rows outside every sequence are neither read nor written. */
+typedef struct {
+    const int32_t *row_start;  /* [n_seqs + 1] */
+    const int32_t *slot;       /* [n_seqs] */
+    const int32_t *ctx_len;    /* [n_seqs] */
+    int n_seqs;                /* at most 4096 */
+    int rows;                  /* rows the row tensors have */
+} mossgpu_seq_batch;
+
+/* Quantises k and v [rows][kv_heads][head_dim] into the cache at their rows' positions.  With a
+ * rope (NULL: none) k turns first, by pos[row] or, where pos is NULL, by its position in the
+ * cache (drafted tokens of one depth share a rotary position, never a cache position); q
+ * [rows][q_heads][head_dim] (NULL: none; needs a rope) turns by the same angle into q_out, which
+ * may be q itself, in the same launch. */
+typedef struct {
+    const void *k, *v, *q;
+    void *q_out;
+    const int32_t *pos;  /* [rows] or NULL */
+    int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int64_t q_row_stride, q_head_stride, q_out_row_stride, q_out_head_stride;
+    int q_heads;
+    int type;            /* of k, v, q and q_out */
+} mossgpu_kv8_append_args;
+int mossgpu_kv8_append(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *seqs, const mossgpu_rope *rope,
+                       const mossgpu_kv8_append_args *args, void *cuda_stream);
+
+/* Reads the batch's positions back: k and v [rows][kv_heads][head_dim] = code * scale, either of
+ * them may be NULL. */
+typedef struct {
+    void *k, *v;
+    int64_t k_row_stride, k_head_stride, v_row_stride, v_head_stride;
+    int type;
+} mossgpu_kv8_read_args;
+int mossgpu_kv8_read(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *seqs, const mossgpu_kv8_read_args *args,
+                     void *cuda_stream);
+
+/* Attention of the batch's rows over the cache, which holds their own K and V already
+ * (mossgpu_kv8_append): row i of a sequence sees its ctx_len positions and, of the sequence's new
+ * rows, those j whose bit (word j / 32, bit j % 32) its mask row sets -- a tree of drafted tokens
+ * sets the bits of a token's ancestors and its own -- or, without a mask, j <= i: one new row is
+ * the decode step of a single token.  New rows past 32 * mask_words are not seen.  q_heads is a
+ * multiple of kv_heads; head h reads kv head h / (q_heads / kv_heads).
+ *   out = sum_j p_j V_j,  p = softmax_j(scale q.K_j);  a row that sees nothing gives zeros
+ * The workspace (any contents, 16-byte aligned, at least mossgpu_attention_kv8_workspace_bytes)
+ * belongs to the call until it has run: two calls that may overlap need two. */
+typedef struct {
+    const void *q;         /* [rows][q_heads][head_dim], turned already */
+    void *out;             /* the same shape and type; must not overlap q */
+    const uint32_t *mask;  /* [rows][mask_words] or NULL */
+    void *workspace;
+    size_t workspace_bytes;
+    int64_t q_row_stride, q_head_stride, out_row_stride, out_head_stride;
+    int q_heads;
+    int type;
+    int mask_words;
+    float scale;
+} mossgpu_attention_kv8_args;
+size_t mossgpu_attention_kv8_workspace_bytes(const mossgpu_kv8_cache *cache, int q_heads, int rows);
+int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *seqs,
+                          const mossgpu_attention_kv8_args *args, void *cuda_stream);
+
+/* Log-probabilities under softmax(logits / temperature) of each row: that of a given token, the
+ * entropy (nats), and the top_k most likely tokens (equal logits: the lower id first) with theirs.
+ * A logit of -inf is a banned token: log-probability -inf, no part of the entropy.  A row of
+ * nothing but -inf gives -inf and entropy 0; a row that holds NaN or +inf gives NaN (NaN logits
+ * rank last).  A negative token asks for none: 0.  A token >= vocab gives NaN. */
+typedef struct {
+    const void *logits;     /* [rows][vocab] */
+    const int32_t *tokens;  /* [rows], or NULL (then logprob is NULL) */
+    float *logprob;         /* [rows] or NULL */
+    float *entropy;         /* [rows] or NULL */
+    int32_t *top_ids;       /* [rows][top_k] or NULL */
+    float *top_logprobs;    /* [rows][top_k] or NULL */
+    int64_t row_stride;
+    int rows, vocab;        /* vocab up to 500000 */
+    int type;               /* of the logits */
+    int top_k;              /* 0 .. min(32, vocab) */
+    float temperature;      /* > 0 */
+} mossgpu_logprob_args;
+int mossgpu_token_logprobs(const mossgpu_logprob_args *args, void *cuda_stream);
+
 /* ---- the audio codec decoder (codes -> 48 kHz interleaved stereo samples) ----
  *
  * Replaces moss::AudioDecoder (reference csrc/include/moss/decoder.h:16-79,
