@@ -1,11 +1,11 @@
 // logprob.cu -- log-probabilities of given tokens, entropy and the most likely tokens of rows of
 // logits (mossgpu_token_logprobs).
 //
-// A row is held in registers, 32 logits a thread, by one CTA of 32 to 1024 threads or by a
-// cluster of up to 16: it is read from HBM once, and the maximum, the sums and the selection all
-// work on what was read.  With x the logits, c = log2(e) / T and M = max x:
-//   Z = sum 2^((x - M) c),  S = sum 2^((x - M) c) (x - M),
-//   log p_t = (x_t - M) / T - ln Z,  entropy = ln Z - S / (T Z).
+// A row is held in registers, 2 or 8 vectors of 16 bytes a thread, by one CTA or by a cluster of
+// up to 16: it is read from HBM once, and the maximum, the sums and the selection all work on what
+// was read.  With x the logits, M = max x, t = (x - M) log2(e) / T:
+//   Z = sum 2^t,  S = sum 2^t t,
+//   log p_i = (x_i - M) / T - ln Z,  entropy = ln Z - ln 2 S / Z.
 // CTAs of a cluster sum against their own maxima; rank 0 merges.
 //
 // Selection: the threads form 32 groups; the k-th largest of the groups' maxima bounds the k-th
@@ -13,13 +13,16 @@
 // -32 ln(1 - k / 32) are expected (9 for k = 8, 31 for k = 20), whatever the distribution, when
 // large logits lie anywhere.  Candidates go to shared memory with their ids and are ranked by
 // counting.  Rows where that does not work -- NaN, or more ties than the buffer holds -- find the
-// exact k-th (logit, id) by bisection instead.
+// exact k-th (logit, id) by bisection instead, over the row as it lies in the cache.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include <math.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "../../include/mossgpu.h"
 #include "op_support.h"
@@ -29,10 +32,10 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLpPerThread = 32;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxCluster = 16;
 constexpr int kLpMaxVocab = 500000;
+constexpr float kLpLn2 = 0.6931471805599453f;
 
 struct LpPart {   // what a CTA of a cluster hands to rank 0
     float top, z, s;
@@ -46,26 +49,133 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     return r;
 }
 
-// Order-preserving bits of a logit; NaN below everything.  (-0 was made +0 when it was read.)
+// Order-preserving bits of a logit (-0 equals +0); NaN below everything.
 __device__ __forceinline__ uint32_t order_bits(float x) {
     if (x != x) return 0u;
-    const uint32_t b = __float_as_uint(x);
+    const uint32_t b = __float_as_uint(x + 0.f);
     return b ^ (b >> 31 ? 0xffffffffu : 0x80000000u);
 }
 __device__ __forceinline__ float order_value(uint32_t k) {
     return k == 0u ? __int_as_float(0x7fffffff) : __uint_as_float(k ^ (k >> 31 ? 0x80000000u : 0xffffffffu));
 }
+__device__ __forceinline__ unsigned long long order_key(float x, int id) {
+    return (unsigned long long)order_bits(x) << 32 | uint32_t(~id);
+}
 
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprobs(const __grid_constant__ mossgpu_logprob_args a, int ctas, int *status) {
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two fp32 operations an instruction.
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 r, a, b;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 r;
+    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 r, a, b;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{\n .reg .b64 a, b, c, r;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+        " fma.rn.f32x2 r, a, b, c;\n mov.b64 {%0, %1}, r;\n}"
+        : "=f"(r.x), "=f"(r.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+
+// Elements 2 i, 2 i + 1 of a vector, and a vector's largest (NaN if it holds one).
+template <typename T>
+__device__ __forceinline__ float2 pair_of(const uint4 &v, int i) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+    if constexpr (sizeof(T) == 4) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    if constexpr (sizeof(T) == 2) {
+        if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2 *>(&w[i]));
+        else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+}
+template <typename T>
+__device__ __forceinline__ float largest(const uint4 &v) {
+    const uint32_t *w = reinterpret_cast<const uint32_t *>(&v);
+    if constexpr (sizeof(T) == 4) {
+        return max_nan(max_nan(__uint_as_float(w[0]), __uint_as_float(w[1])), max_nan(__uint_as_float(w[2]), __uint_as_float(w[3])));
+    } else if constexpr (std::is_same<T, __half>::value) {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&v);
+        const float2 m = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+        return max_nan(m.x, m.y);
+    } else {
+        const __nv_bfloat162 *h = reinterpret_cast<const __nv_bfloat162 *>(&v);
+        const float2 m = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+        return max_nan(m.x, m.y);
+    }
+}
+
+// Exact selection of a CTA's first k (logit, id) of its share of a row into `cand`: the order bits
+// of the k-th largest by bisection, then the id among its ties.  Returns how many there are.
+template <typename T, int NT, typename IdOf>
+__device__ __noinline__ int select_exact(const T *x_row, int vocab, int top_k, int vectors, IdOf id_of, int *sum, unsigned long long *cand) {
     constexpr int VE = 16 / int(sizeof(T));
-    constexpr int NV = kLpPerThread / VE;
+    const auto count = [&](auto &&in) {
+        int n = 0;
+        for (int v = 0; v < vectors; ++v)
+            for (int i = 0; i < VE; ++i) {
+                const int id = id_of(v, i);
+                if (id >= 0 && id < vocab) n += in(order_bits(float(x_row[id])), id) ? 1 : 0;
+            }
+        __syncthreads();
+        if (threadIdx.x == 0) *sum = 0;
+        __syncthreads();
+        n = __reduce_add_sync(0xffffffffu, n);
+        if ((threadIdx.x & 31) == 0) atomicAdd(sum, n);
+        __syncthreads();
+        return *sum;
+    };
+    const int k = min(top_k, count([](uint32_t, int) { return true; }));
+    uint32_t key = 0;  // largest key that at least k logits reach
+    for (int bit = 31; bit >= 0; --bit) {
+        const uint32_t trial = key | 1u << bit;
+        if (count([=](uint32_t b, int) { return b >= trial; }) >= k) key = trial;
+    }
+    int last = 0;  // smallest id up to which the ties complete the k
+    for (int bit = 19; bit >= 0; --bit) {
+        const int trial = last + (1 << bit);  // are the ids below `trial` too few?
+        if (count([=](uint32_t b, int id) { return b > key || (b == key && id < trial); }) < k) last = trial;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) *sum = 0;
+    __syncthreads();
+    if (k > 0)
+        for (int v = 0; v < vectors; ++v)
+            for (int i = 0; i < VE; ++i) {
+                const int id = id_of(v, i);
+                if (id < 0 || id >= vocab) continue;
+                const float x = float(x_row[id]);
+                const uint32_t b = order_bits(x);
+                if (b > key || (b == key && id <= last)) cand[atomicAdd(sum, 1)] = order_key(x, id);
+            }
+    __syncthreads();
+    return *sum;
+}
+
+// NT threads hold NV vectors each; `ctas` CTAs a row.
+template <typename T, int NT, int NV>
+__global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT) k_token_logprobs(
+    const __grid_constant__ mossgpu_logprob_args a, int ctas, int *status) {
+    constexpr int VE = 16 / int(sizeof(T));
+    // candidates a CTA ranks; 32 groups of a uniform row give about 130 at k = 32
+    constexpr int kCandidates = NT == 32 ? 256 : 512;
     __shared__ __align__(16) float group_top[32];
     __shared__ float2 warp_sums[NT / 32];
-    // candidates a CTA ranks; 32 groups of a uniform row give about 130 at k = 32
-    constexpr int kLpCandidates = NT == 32 ? 256 : 512;
-    __shared__ unsigned long long cand[kLpCandidates];
-    __shared__ int n_cand, n_cand_old;
+    __shared__ unsigned long long cand[kCandidates];
+    __shared__ int n_cand;
     __shared__ LpPart parts[NT < 512 ? 1 : kLpMaxCluster];  // clusters have CTAs of 512 threads or more
     const int tid = threadIdx.x, lane = tid & 31;
     const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas;
@@ -75,30 +185,27 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprob
     if (tid == 0) n_cand = 0;
 
     // ---- the row; vector v holds elements v VE - lead ..
-    float x[NV][VE];
-    const auto id_of = [&](int v, int i) { return ((v * ctas + rank) * NT + tid) * VE - lead + i; };
+    uint4 x[NV];
+    const auto id_of = [=](int v, int i) { return ((v * ctas + rank) * NT + tid) * VE - lead + i; };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int e0 = id_of(v, 0);
         if (e0 >= 0 && e0 + VE <= a.vocab) {
-            const uint4 raw = __ldg(reinterpret_cast<const uint4 *>(x_row + e0));
-            const T *e = reinterpret_cast<const T *>(&raw);
-#pragma unroll
-            for (int i = 0; i < VE; ++i) x[v][i] = float(e[i]) + 0.f;
+            x[v] = __ldg(reinterpret_cast<const uint4 *>(x_row + e0));
         } else {
+            T e[VE];
 #pragma unroll
-            for (int i = 0; i < VE; ++i)
-                x[v][i] = e0 + i >= 0 && e0 + i < a.vocab ? float(x_row[e0 + i]) + 0.f : -INFINITY;
+            for (int i = 0; i < VE; ++i) e[i] = e0 + i >= 0 && e0 + i < a.vocab ? x_row[e0 + i] : T(-INFINITY);
+            memcpy(&x[v], e, 16);
         }
     }
-    float mine = -INFINITY;
+    float mine = largest<T>(x[0]);
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+    for (int v = 1; v < NV; ++v) mine = max_nan(mine, largest<T>(x[v]));
+    float group = mine;
 #pragma unroll
-        for (int i = 0; i < VE; ++i) mine = max_nan(mine, x[v][i]);
-#pragma unroll
-    for (int o = 1; o < NT / 32; o <<= 1) mine = max_nan(mine, __shfl_xor_sync(0xffffffffu, mine, o));
-    if (tid % (NT / 32) == 0) group_top[tid / (NT / 32)] = mine;
+    for (int o = 1; o < NT / 32; o <<= 1) group = max_nan(group, __shfl_xor_sync(0xffffffffu, group, o));
+    if (tid % (NT / 32) == 0) group_top[tid / (NT / 32)] = group;
     __syncthreads();
 
     // ---- every warp: the CTA's maximum, and the k-th largest of the 32 groups' maxima
@@ -119,103 +226,55 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprob
             above += q.w > g || (q.w == g && 4 * j + 3 < lane);
         }
         bound = __shfl_sync(0xffffffffu, g, __ffs(__ballot_sync(0xffffffffu, above == a.top_k - 1)) - 1);
+        // ---- candidates: few threads have any
+        const bool few = bound == -INFINITY;  // fewer than k groups hold anything: every finite logit, and the first ids
+        if (mine >= bound) {
+#pragma unroll
+            for (int v = 0; v < NV; ++v) {
+                uint32_t in = 0;
+#pragma unroll
+                for (int i = 0; i < VE / 2; ++i) {
+                    const float2 f = pair_of<T>(x[v], i);
+                    if (few ? f.x > bound : f.x >= bound) in |= 1u << (2 * i);
+                    if (few ? f.y > bound : f.y >= bound) in |= 2u << (2 * i);
+                }
+                const int e0 = id_of(v, 0);
+                if (few && e0 < a.top_k) {
+                    for (int i = 0; i < VE; ++i)
+                        if (e0 + i >= 0 && e0 + i < a.top_k) in |= 1u << i;
+                }
+                for (; in; in &= in - 1) {
+                    const int id = e0 + __ffs(in) - 1, at = atomicAdd(&n_cand, 1);
+                    if (at < kCandidates) cand[at] = order_key(float(x_row[id]), id);
+                }
+            }
+        }
     }
 
-    // ---- sums, and candidates
-    float z = 0.f, s = 0.f;
+    // ---- sums
+    float2 z = make_float2(0.f, 0.f), s = z;
     const float c = 1.4426950408889634f / a.temperature;
-    const bool few = bound == -INFINITY;  // fewer than k groups hold anything: every finite logit, and the first ids
+    const float2 c2 = make_float2(c, c), off = make_float2(-top, -top);
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) {
-            const float d = x[v][i] - top;
-            float e;
-            asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * c));
-            z += e;
-            s = fmaf(e, fmaxf(d, -3e38f), s);  // 0 * infinity stays out of the sum
+        for (int i = 0; i < VE / 2; ++i) {
+            float2 t = mul2(add2(pair_of<T>(x[v], i), off), c2), e;
+            t.x = fmaxf(t.x, -200.f), t.y = fmaxf(t.y, -200.f);  // 2^-200 is 0, and 0 * infinity stays out of the sum
+            e.x = ex2(t.x), e.y = ex2(t.y);
+            z = add2(z, e);
+            s = fma2(e, t, s);
         }
-    if (a.top_k > 0 && sound) {
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                bool in = x[v][i] >= bound;
-                if (few) {
-                    const int id = id_of(v, i);
-                    in = id >= 0 && id < a.vocab && (x[v][i] > -INFINITY || id < a.top_k);
-                }
-                if (in) {
-                    const int at = atomicAdd(&n_cand, 1);
-                    if (at < kLpCandidates)
-                        cand[at] = (unsigned long long)order_bits(x[v][i]) << 32 | uint32_t(~id_of(v, i));
-                }
-            }
-    }
+    z.x += z.y, s.x += s.y;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        z += __shfl_xor_sync(0xffffffffu, z, o);
-        s += __shfl_xor_sync(0xffffffffu, s, o);
+        z.x += __shfl_xor_sync(0xffffffffu, z.x, o);
+        s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
     }
-    if (lane == 0) warp_sums[tid >> 5] = make_float2(z, s);
+    if (lane == 0) warp_sums[tid >> 5] = make_float2(z.x, s.x);
     __syncthreads();
-
-    if (a.top_k > 0 && (!sound || n_cand > kLpCandidates)) {
-        // ---- exact selection: bisect the order bits of the k-th largest, then the id among its ties
-        int valid = 0;
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) valid += id_of(v, i) >= 0 && id_of(v, i) < a.vocab;
-        const auto block_sum = [&](int n) {
-            __syncthreads();
-            if (tid == 0) n_cand_old = 0;
-            __syncthreads();
-            n = __reduce_add_sync(0xffffffffu, n);
-            if (lane == 0) atomicAdd(&n_cand_old, n);
-            __syncthreads();
-            return n_cand_old;
-        };
-        const int k = min(a.top_k, block_sum(valid));
-        uint32_t key = 0;  // largest key that at least k logits reach
-        for (int bit = 31; bit >= 0; --bit) {
-            const uint32_t trial = key | 1u << bit;
-            int n = 0;
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int i = 0; i < VE; ++i)
-                    n += order_bits(x[v][i]) >= trial && id_of(v, i) >= 0 && id_of(v, i) < a.vocab;
-            if (block_sum(n) >= k) key = trial;
-        }
-        int last = 0;  // smallest id up to which the ties complete the k
-        for (int bit = 19; bit >= 0; --bit) {
-            const int trial = last + (1 << bit);  // are the ids below `trial` too few?
-            int n = 0;
-#pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int i = 0; i < VE; ++i) {
-                    const int id = id_of(v, i);
-                    const uint32_t b = order_bits(x[v][i]);
-                    n += id >= 0 && id < a.vocab && (b > key || (b == key && id < trial));
-                }
-            if (block_sum(n) < k) last = trial;
-        }
-        __syncthreads();
-        if (tid == 0) n_cand = 0;
-        __syncthreads();
-#pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int i = 0; i < VE; ++i) {
-                const int id = id_of(v, i);
-                const uint32_t b = order_bits(x[v][i]);
-                if (k > 0 && id >= 0 && id < a.vocab && (b > key || (b == key && id <= last)))
-                    cand[atomicAdd(&n_cand, 1)] = (unsigned long long)b << 32 | uint32_t(~id);
-            }
-        __syncthreads();
-    }
+    int n = n_cand;
+    if (a.top_k > 0 && (!sound || n > kCandidates)) n = select_exact<T, NT>(x_row, a.vocab, a.top_k, NV, id_of, &n_cand, cand);
 
     // ---- the CTA's share
     LpPart *mine_part = &parts[rank];
@@ -223,7 +282,6 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprob
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // rank 0 runs, its shared memory may be written
         mine_part = cg::this_cluster().map_shared_rank(&parts[rank], 0);
     }
-    const int n = min(n_cand, kLpCandidates);
     for (int i = tid; i < n; i += NT) {
         const unsigned long long key = cand[i];
         int r = 0;
@@ -233,7 +291,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprob
     if (tid < 32) {
         float2 t = tid < NT / 32 ? warp_sums[tid] : make_float2(0.f, 0.f);
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) {
+        for (int o = NT / 64; o > 0; o >>= 1) {
             t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
             t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
         }
@@ -247,21 +305,21 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprob
     }
 
     // ---- rank 0: the row
-    float m = -INFINITY;
-    for (int r = 0; r < ctas; ++r) m = max_nan(m, parts[r].top);
-    float zz = 0.f, ss = 0.f;
-    for (int r = 0; r < ctas; ++r) {
-        const LpPart &q = parts[r];
-        if (q.top == -INFINITY) continue;  // nothing there
-        const float d = q.top - m;         // sums against the part's own maximum
-        float e;
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(d * c));
-        zz = fmaf(q.z, e, zz);
-        ss = fmaf(e, fmaf(q.z, fmaxf(d, -1e30f), q.s), ss);
+    float m = parts[0].top, zz = parts[0].z, ss = parts[0].s;
+    if (ctas > 1) {
+        for (int r = 1; r < ctas; ++r) m = max_nan(m, parts[r].top);
+        zz = ss = 0.f;
+        for (int r = 0; r < ctas; ++r) {
+            const LpPart &q = parts[r];
+            if (q.top == -INFINITY) continue;  // nothing there
+            const float t = fmaxf((q.top - m) * c, -200.f), e = ex2(t);  // sums against the part's own maximum
+            zz = fmaf(q.z, e, zz);
+            ss = fmaf(e, fmaf(q.z, t, q.s), ss);
+        }
     }
-    const float inv_t = 1.f / a.temperature;
     const bool empty = m == -INFINITY, bad = !(m < INFINITY);  // NaN or +inf
-    const float ln_z = logf(zz), nan = __int_as_float(0x7fffffff);
+    const float log_z = log2f(zz), ln_z = log_z * kLpLn2, inv_t = 1.f / a.temperature, nan = __int_as_float(0x7fffffff);
+    // (v - m) / T rather than ln 2 t: t of the type's lowest value is past the range of fp32
     const auto logprob = [&](float v) { return bad ? nan : v == -INFINITY ? -INFINITY : (v - m) * inv_t - ln_z; };
     if (tid == 0) {
         if (a.logprob) {
@@ -275,36 +333,44 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 24 : 1024 / NT) k_token_logprob
             }
             a.logprob[row] = lp;
         }
-        if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.f : ln_z - ss / zz * inv_t;
+        if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.f : (log_z - ss / zz) * kLpLn2;
     }
-    if (a.top_k > 0) {
-        // merge the parts' sorted lists: an entry's rank is its own plus, of every other part, how many are larger
-        for (int i = tid; i < ctas * kLpMaxTop; i += NT) {
-            const int r = i / kLpMaxTop, j = i % kLpMaxTop;
-            if (j >= parts[r].count) continue;
-            const unsigned long long key = parts[r].best[j];
-            int at = j;
-            for (int q = 0; q < ctas; ++q) {
-                if (q == r) continue;
-                int lo = 0, hi = parts[q].count;
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (parts[q].best[mid] > key) lo = mid + 1; else hi = mid;
-                }
-                at += lo;
+    if (a.top_k == 0) return;
+    if (ctas == 1) {
+        for (int i = tid; i < a.top_k; i += NT) {  // a CTA has the whole row: top_k <= vocab entries are there
+            const unsigned long long key = parts[0].best[i];
+            const int64_t to = int64_t(row) * a.top_k + i;
+            if (a.top_ids) a.top_ids[to] = int32_t(~uint32_t(key));
+            if (a.top_logprobs) a.top_logprobs[to] = logprob(order_value(uint32_t(key >> 32)));
+        }
+        return;
+    }
+    // merge the parts' sorted lists: an entry's rank is its own plus, of every other part, how many are larger
+    for (int i = tid; i < ctas * kLpMaxTop; i += NT) {
+        const int r = i / kLpMaxTop, j = i % kLpMaxTop;
+        if (j >= parts[r].count) continue;
+        const unsigned long long key = parts[r].best[j];
+        int at = j;
+        for (int q = 0; q < ctas; ++q) {
+            if (q == r) continue;
+            int lo = 0, hi = parts[q].count;
+            while (lo < hi) {
+                const int mid = (lo + hi) >> 1;
+                if (parts[q].best[mid] > key) lo = mid + 1; else hi = mid;
             }
-            if (at < a.top_k) {
-                const int64_t to = int64_t(row) * a.top_k + at;
-                if (a.top_ids) a.top_ids[to] = int32_t(~uint32_t(key));
-                if (a.top_logprobs) a.top_logprobs[to] = logprob(order_value(uint32_t(key >> 32)));
-            }
+            at += lo;
+        }
+        if (at < a.top_k) {
+            const int64_t to = int64_t(row) * a.top_k + at;
+            if (a.top_ids) a.top_ids[to] = int32_t(~uint32_t(key));
+            if (a.top_logprobs) a.top_logprobs[to] = logprob(order_value(uint32_t(key >> 32)));
         }
     }
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int NV>
 cudaError_t launch(const mossgpu_logprob_args &a, int ctas, int *status, cudaStream_t st) {
-    auto *kernel = k_token_logprobs<T, NT>;
+    auto *kernel = k_token_logprobs<T, NT, NV>;
     if (ctas > 8) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
@@ -324,18 +390,23 @@ cudaError_t launch(const mossgpu_logprob_args &a, int ctas, int *status, cudaStr
 
 template <typename T>
 cudaError_t dispatch(const mossgpu_logprob_args &a, int *status, cudaStream_t st) {
-    // threads a row needs at 32 logits each, one vector more where rows start off a 16-byte boundary
+    // vectors a row touches: one more where rows start off a 16-byte boundary
     constexpr int VE = 16 / int(sizeof(T));
-    const int need = (a.vocab + VE - 1 + kLpPerThread - 1) / kLpPerThread;
-    if (need <= 32 || (a.vocab <= 1024 && reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && a.row_stride % VE == 0))
-        return launch<T, 32>(a, 1, status, st);
-    if (need <= 128) return launch<T, 128>(a, 1, status, st);
-    if (need <= 512) return launch<T, 512>(a, 1, status, st);
-    int ctas = 2;
-    while (ctas < 8 && need > 512 * ctas) ctas *= 2;
-    if (need <= 512 * ctas) return launch<T, 512>(a, ctas, status, st);
-    while (ctas < kLpMaxCluster && need > 1024 * ctas) ctas *= 2;
-    return launch<T, 1024>(a, ctas, status, st);
+    const bool even = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (a.row_stride % VE == 0 || a.rows == 1);
+    const int n = (a.vocab + (even ? 0 : VE - 1) + VE - 1) / VE;
+    // Two vectors a thread where all rows' threads are resident at once: a row's latency is what its
+    // longest thread does.  Eight otherwise: the per-row work is spread over more logits.
+    if (int64_t(a.rows) * n <= int64_t(2) * 148 * 1024) {
+        if (n <= 2 * 128) return launch<T, 128, 2>(a, 1, status, st);
+        for (int ctas = 1; ctas <= kLpMaxCluster; ctas *= 2)
+            if (n <= 2 * 512 * ctas) return launch<T, 512, 2>(a, ctas, status, st);
+    }
+    if (n <= 8 * 32) return launch<T, 32, 8>(a, 1, status, st);
+    if (n <= 8 * 128) return launch<T, 128, 8>(a, 1, status, st);
+    int ctas = 1;
+    while (ctas < kLpMaxCluster && n > 8 * 512 * ctas) ctas *= 2;
+    if (n <= 8 * 512 * ctas) return launch<T, 512, 8>(a, ctas, status, st);
+    return launch<T, 1024, 8>(a, ctas, status, st);
 }
 
 }  // namespace

@@ -345,7 +345,7 @@ typedef struct {
 /* A ragged batch: sequence s owns rows row_start[s] .. row_start[s + 1] - 1 of the row tensors
  * (row_start ascends; a sequence may own none), lives in slot[s] and has ctx_len[s] positions in
  * the cache already: its i-th row is position ctx_len[s] + i.  The slots of a call are distinct.
- * Rows outside every sequence are neither read nor written. */
+ * Rows outside every sequence are left as they are. */
 typedef struct {
     const int32_t *row_start;  /* [n_seqs + 1] */
     const int32_t *slot;       /* [n_seqs] */
