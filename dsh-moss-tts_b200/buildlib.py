@@ -9,7 +9,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libmossgpu.so"
 SOURCES = ["engine.cu", "ops.cu", "kv8.cu", "logprob.cu", "codec.cu", "capi.cpp"]
-HEADERS = ["types.h", "kernels.cuh", "gemm_tc.cuh", "attn_tc.cuh", "local_fused.cuh", "layer_small.cuh", "engine.h", "op_support.h",
+HEADERS = ["types.h", "kernels.cuh", "gemm_tc.cuh", "attn_tc.cuh", "local_fused.cuh", "layer_small.cuh", "engine.h", "op_support.h", "f32x2.cuh",
            "kv8_index.h", "rope_kv8.cuh", "attn_kv8.cuh", "../../include/mossgpu.h"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 FLAGS = ["--threads", "0", "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17",

@@ -1,30 +1,38 @@
 // attn_kv8.cuh -- attention of one or a few new rows a sequence over the 8-bit paged cache.
 //
-// Work.  A unit is (sequence, kv head, block of kTileRows query rows); its rows are the
-// sequence's new rows times the query heads of the group, so a cache byte serves all of them.  A
-// unit's positions come in tiles of 32 (two pages).  All tiles of all units, in order, are cut
-// into equal runs, one per warp of the grid: however ragged the batch is, every warp has the same
-// work.  A warp that has a whole unit writes its rows; a unit cut between warps leaves partial
-// sums in the workspace, which k_attn_kv8_join (a dependent launch) merges in a fixed order, so
-// that a result does not depend on timing.
+// DIRECT: a CTA has a whole unit, its warps the tiles in turn; no plan, no second launch.
 //
-// A tile.  The warp's own ring of tiles in shared memory is filled by cp.async (16 bytes a lane,
-// no barrier but the warp's own).  S = q K^T and o += w V are mma.sync m16n8k16 products in fp16,
-// in which every 8-bit code is exact.  Which element of the head dimension is the k-th of a
-// product, and which position is the n-th, is free as long as both operands agree; here a lane
-// takes 16 consecutive codes of a K row and, of four V rows, consecutive codes too, so that codes
-// go from shared memory to a fragment by wide loads and conversions alone.  The scales of a
-// position multiply its score (K) and its weight (V) in fp32.
+// Work otherwise.  A unit is (sequence, kv head, block of query rows); its rows are the sequence's
+// new rows times the query heads of the group, so a cache byte serves all of them.  A unit's
+// positions come in tiles of 32 (two pages).  All tiles of one head, in order, are cut into equal
+// runs, one run of one head per warp of the grid: however ragged the batch is, every warp has the
+// same work.  The heads of a run go to neighbouring warps, since a page's heads lie side by side:
+// 512 long sequences take 372 us with every head's tiles in a warp of its own somewhere, as the pages'
+// address translations are then missed for every 1 KB block.  A warp that has a whole unit writes its
+// rows; a unit cut between warps leaves partial sums in the workspace, which k_attn_kv8_join (a
+// dependent launch) merges in a fixed order, so that a result does not depend on timing.
+//
+// A tile.  K, V and their scales of the pages (each contiguous) are copied to a stage of the warp's own
+// ring in shared memory, 16 bytes a lane (bulk copies of 1 KB need more instructions: they are issued
+// one lane after the other).  No barrier but the warp's own.  S = q K^T
+// and o += w V are mma.sync m16n8k16 products in fp16, in which every 8-bit code is exact.  Which
+// element of the head dimension is the k-th of a product, and which position is the n-th, is free as
+// long as both operands agree.  Here a lane takes 16 consecutive codes of a K row, the same columns of
+// four neighbouring V rows, and those four positions' scales as one vector, so that codes go from
+// shared memory to a fragment by wide loads and conversions alone.  The scales of a position multiply
+// its score (K) and its weight (V) in fp32.
 //
 // Precision.  A query row is scaled by a power of two to [128, 256) and rounded to fp16, exact for
-// bf16 and fp16 inputs.  For bf16 outputs the weights w = p sv 2^(13 - E), E the exponent of the
-// largest V scale so far, are rounded to fp16 as well (2^-11 against the output's 2^-8), 16 rows
-// a product.  For fp32 and fp16 outputs both are split into an upper and a lower fp16 part (22
-// bits) that occupy rows g and g + 8 of the same product, 8 rows a product; since the tensor
-// cores truncate when they accumulate, such products start from zero and are added in fp32.
-// Statistics, sums and partials are fp32.
+// bf16 and fp16 inputs.  Weights are taken relative to R = m - (140 - E), m the running maximum of the
+// scores (in log2) and E the exponent of the largest V scale so far: w = 2^(s - R) sv < 2^14 fits
+// fp16 whatever the scales are.  For bf16 outputs w is rounded to fp16 (2^-11 against the output's
+// 2^-8), 16 rows a product.  For fp32 and fp16 outputs q and w are split into an upper and a lower
+// fp16 part (22 bits) that occupy rows g and g + 8 of the same product, 8 rows a product; since the
+// tensor cores truncate when they accumulate, such products start from zero every tile and are added
+// in fp32.  Statistics, sums and partials are fp32.
 #pragma once
 
+#include "f32x2.cuh"
 #include "rope_kv8.cuh"
 
 namespace mossgpu {
@@ -41,27 +49,67 @@ struct Ak8Shape {
     static constexpr int kRing = kStage * kStages * kWarps;    // 208,896 and 202,752 bytes
 };
 
+// k_attn_kv8_few: pages of a tile, warps of a CTA, stages of a warp's ring
+template <int D>
+struct Ak8Few {
+    static constexpr int kPages = 2;
+    static constexpr int kBlock = 16 * D;
+    static constexpr int kStage = kPages * (2 * kBlock + 128);
+    static constexpr int kWarps = D == 64 ? 16 : 12;
+    static constexpr int kStages = D == 64 ? 3 : 2;
+    static constexpr int kRing = kStage * kStages * kWarps;
+};
+
 struct AttnKv8 {
     mossgpu_kv8_cache cache;
     mossgpu_seq_batch seqs;
     mossgpu_attention_kv8_args a;
     int group;       // query heads per kv head
-    int workers;     // warps of the grid
+    int runs;        // most runs a head's tiles are cut into: runs * kv_heads <= warps of the grid
     int tile_rows;   // rows of a unit
     int part_rows;   // rows a partial keeps
     int vec_q, vec_out;
     uint32_t *plan;  // [n_seqs + 1] tiles (over row blocks, per kv head) before a sequence; then [n_seqs] tiles of one block
-    float *part;     // [2 * workers][part_rows][head_dim + 4]: sums, then m (log2 units) and l
+    float *part;     // [2 * runs * kv_heads][part_rows][head_dim + 4]: sums, then R and l
     int *status;
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Copies NP pages of a head (id: lane i < NP has page i's, -1 for none) to a stage:
+// K pages, V pages, then the scales as [k, v][page][16].
+template <int D, int NP>
+__device__ __forceinline__ void copy_pages(const mossgpu_kv8_cache &c, int head, uint32_t dst, int id) {
+    constexpr int kBlock = 16 * D;
+    const int lane = threadIdx.x & 31;
+    const uint32_t page_bytes = uint32_t(2 * kBlock) * uint32_t(c.kv_heads);
+#pragma unroll
+    for (int pg = 0; pg < NP; ++pg) {
+        const int page = __shfl_sync(0xffffffffu, id, pg);
+        if (page >= 0) {
+            const uint8_t *k = static_cast<const uint8_t *>(c.codes) + uint64_t(uint32_t(page)) * page_bytes + uint32_t(head * kBlock + lane * 16);
+            const uint8_t *v = k + page_bytes / 2;
+#pragma unroll
+            for (int i = 0; i < kBlock / 512; ++i) {
+                cp_async16(dst + pg * kBlock + lane * 16 + i * 512, k + i * 512);
+                cp_async16(dst + (NP + pg) * kBlock + lane * 16 + i * 512, v + i * 512);
+            }
+        }
+    }
+    // lane: K or V (lane / (4 NP)), page (lane / 4), 4 scales
+    const int page = __shfl_sync(0xffffffffu, id, (lane >> 2) & (NP - 1));
+    if (lane < 8 * NP && page >= 0) {
+        const float *s = c.scales + uint64_t(uint32_t(page)) * uint32_t(2 * kKv8Page * c.kv_heads) +
+                         uint32_t(((lane >= 4 * NP ? c.kv_heads : 0) + head) * kKv8Page + (lane & 3) * 4);
+        cp_async16(dst + 2 * NP * kBlock + lane * 16, s);
+    }
 }
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -71,13 +119,21 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// the same from zero
+__device__ __forceinline__ void mma16816_0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                           uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
 __device__ __forceinline__ uint32_t half2_bits(__half2 h) { return *reinterpret_cast<uint32_t *>(&h); }
-__device__ __forceinline__ uint32_t pack2(float a, float b) { return half2_bits(__floats2half2_rn(a, b)); }
-// the fp16 parts of (a, b): upper returned, lower = what the upper leaves
-__device__ __forceinline__ uint32_t split2(float a, float b, uint32_t *lower) {
-    const __half2 h = __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t pack2(float2 x) { return half2_bits(__float22half2_rn(x)); }
+// the fp16 parts of a pair: upper returned, lower = what the upper leaves
+__device__ __forceinline__ uint32_t split2(float2 x, uint32_t *lower) {
+    const __half2 h = __float22half2_rn(x);
     const float2 f = __half22float2(h);
-    *lower = pack2(a - f.x, b - f.y);
+    *lower = pack2(make_float2(x.x - f.x, x.y - f.y));
     return half2_bits(h);
 }
 
@@ -98,24 +154,7 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &lo, uint32_t &hi
     }
 }
 
-// 16-byte granule `gr` of row r (0..15) of a block, in the order that makes the K and the V reads
-// of a tile free of bank conflicts.
-template <int D>
-__device__ __forceinline__ int granule(int r, int gr) {
-    const int x = D == 64 ? (r & 2) : (((r & 1) << 2) | (r & 2));
-    return r * (D / 16) + (gr ^ x);
-}
-
-// Position, within a page, of the n-th column of the tau-th product (n = 2 t + e).
-__device__ __forceinline__ int page_row(int tau, int t, int e) { return ((t + e) & 3) + 4 * (2 * tau + e); }
-
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
-
-__device__ __forceinline__ float exp2_approx(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
 
 // 8 elements of a row of q, whatever its type
 __device__ __forceinline__ void load_q8(const void *q, int type, bool vec, int64_t at, float (&x)[8]) {
@@ -135,156 +174,251 @@ __device__ __forceinline__ void store_out8(void *o, int type, bool vec, int64_t 
         store8(static_cast<__nv_bfloat16 *>(o) + at, vec, x);
 }
 
-// Worker w has the tiles [total w / n, total (w + 1) / n); n <= total.
-__device__ __forceinline__ int64_t run_begin(int64_t total, int n, int w) { return total * w / n; }
+// Run r of n has the tiles [total r / n, total (r + 1) / n); n <= total.
+__device__ __forceinline__ int64_t run_begin(int64_t total, int n, int r) { return total * r / n; }
 __device__ __forceinline__ int run_of(int64_t total, int n, int64_t g) { return int(((g + 1) * n - 1) / total); }
-__device__ __forceinline__ int runs_used(int64_t total, int workers) { return int(total < workers ? total : workers); }
+__device__ __forceinline__ int runs_used(int64_t total, int runs) { return int(total < runs ? total : runs); }
 
-template <int D, int FORMAT, bool SPLIT>
+// Tiles (of TILE positions, over blocks of ROWS query rows, per kv head) before each sequence, in
+// shared memory, and, from CTA 0, in the workspace for k_attn_kv8_join.  Returns those of the batch.
+template <int ROWS, int TILE, int WARPS>
+__device__ __forceinline__ int64_t plan_tiles(const AttnKv8 &p, uint32_t *plan) {
+    __shared__ uint32_t warp_sum[WARPS];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n_seqs = p.seqs.n_seqs;
+    uint32_t before = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += WARPS * 32) {
+        const int s = s0 + int(threadIdx.x);
+        uint32_t mine = 0;
+        if (s < n_seqs) {
+            const RowRange r = kv8_rows(__ldg(p.seqs.row_start + s), __ldg(p.seqs.row_start + s + 1), p.seqs.rows);
+            const int slot = __ldg(p.seqs.slot + s), ctx = __ldg(p.seqs.ctx_len + s);
+            int status = 0;
+            if (r.r1 > r.r0) {
+                const SeqSpan span = kv8_span(p.cache, slot, ctx, r.r1 - r.r0, &status);
+                const uint32_t tiles = span.total > 0 ? (span.total + TILE - 1) / TILE : 1;
+                mine = tiles * uint32_t(((r.r1 - r.r0) * p.group + ROWS - 1) / ROWS);
+                if (blockIdx.x == 0) p.plan[n_seqs + 1 + s] = tiles;
+            }
+            if (blockIdx.x == 0) op_report(p.status, status);
+        }
+        uint32_t sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        if (lane == 31) warp_sum[warp] = sum;
+        __syncthreads();
+        uint32_t base = before, all = 0;
+        for (int w = 0; w < WARPS; ++w) {
+            if (w < warp) base += warp_sum[w];
+            all += warp_sum[w];
+        }
+        if (s < n_seqs) plan[s] = base + sum - mine;
+        before += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) plan[n_seqs] = before;
+    __syncthreads();
+    if (blockIdx.x == 0)
+        for (int s = threadIdx.x; s <= n_seqs; s += WARPS * 32) p.plan[s] = plan[s];
+    return int64_t(plan[n_seqs]);
+}
+
+// This warp's run, as tiles [g, g_end) of a head: the (run, head) pairs are dealt to the CTAs evenly and in order.
+struct Run {
+    int64_t g, g_end;
+    int item, head;
+};
+template <int WARPS>
+__device__ __forceinline__ bool warp_run(const AttnKv8 &p, int64_t total, Run &w) {
+    const int H = p.cache.kv_heads, used = runs_used(total, p.runs);
+    const int64_t items = int64_t(used) * H;
+    const int lo = int(items * blockIdx.x / gridDim.x), hi = int(items * (blockIdx.x + 1) / gridDim.x);
+    w.item = lo + int(threadIdx.x >> 5);
+    if (w.item >= hi) return false;
+    const int r = w.item / H;
+    w.head = w.item - r * H;
+    w.g = run_begin(total, used, r);
+    w.g_end = run_begin(total, used, r + 1);
+    return true;
+}
+
+// The unit that tile g of a head belongs to, and its tiles [t0, t1) in a run that ends at g_end.
+struct Unit {
+    RowRange rr;
+    SeqSpan span;
+    int head, block, tiles, t0, t1, n_rows, n_pages;
+    const int32_t *table;
+};
+// Sequence s's share of it; returns the status of its span.
+__device__ __forceinline__ int fill_unit(const AttnKv8 &p, int s, int tile, Unit &u) {
+    u.rr = kv8_rows(__ldg(p.seqs.row_start + s), __ldg(p.seqs.row_start + s + 1), p.seqs.rows);
+    const int slot = __ldg(p.seqs.slot + s);
+    int status = 0;
+    u.span = kv8_span(p.cache, slot, __ldg(p.seqs.ctx_len + s), u.rr.r1 - u.rr.r0, &status);
+    u.tiles = u.span.total > 0 ? (u.span.total + tile - 1) / tile : 1;
+    u.n_rows = (u.rr.r1 - u.rr.r0) * p.group;
+    u.table = p.cache.page_table + size_t(u.span.total > 0 ? slot : 0) * p.cache.pages_per_slot;
+    u.n_pages = (u.span.total + kKv8Page - 1) / kKv8Page;
+    return status;
+}
+// E elements of an output row, times f
+template <int E>
+__device__ __forceinline__ void store_row(const AttnKv8 &p, int row, int head, int at, const float (&y)[E], float f) {
+    const int64_t to = int64_t(row) * p.a.out_row_stride + int64_t(head) * p.a.out_head_stride + at;
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+        if (p.a.type == MOSSGPU_F32)
+            static_cast<float *>(p.a.out)[to + i] = y[i] * f;
+        else if (p.a.type == MOSSGPU_F16)
+            static_cast<__half *>(p.a.out)[to + i] = __float2half_rn(y[i] * f);
+        else
+            static_cast<__nv_bfloat16 *>(p.a.out)[to + i] = __float2bfloat16_rn(y[i] * f);
+    }
+}
+__device__ __forceinline__ Unit find_unit(const AttnKv8 &p, const uint32_t *plan, const Run &w, int tile) {
+    int lo = 0, hi = p.seqs.n_seqs;  // the last sequence that begins at or before g: it has tiles
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (int64_t(plan[mid]) <= w.g) lo = mid; else hi = mid;
+    }
+    Unit u;
+    fill_unit(p, lo, tile, u);  // its status is reported by plan_tiles
+    u.head = w.head;
+    const uint32_t at = uint32_t(w.g) - plan[lo];
+    u.block = int(at / uint32_t(u.tiles));
+    u.t0 = int(at - uint32_t(u.block) * uint32_t(u.tiles));
+    u.t1 = int(min(int64_t(u.tiles), u.t0 + (w.g_end - w.g)));
+    return u;
+}
+
+// Unit `index` of the batch where a CTA has a whole one: block (index / heads) of all sequences' blocks
+// of ROWS query rows.  n_rows is 0 past the last.
+template <int ROWS>
+__device__ __forceinline__ Unit direct_unit(const AttnKv8 &p, int index, int tile, int *status) {
+    const int lane = threadIdx.x & 31, H = p.cache.kv_heads, want = index / H;
+    Unit u;
+    u.n_rows = 0;
+    int before = 0;
+    for (int s0 = 0; s0 < p.seqs.n_seqs; s0 += 32) {
+        int blocks = 0;
+        if (s0 + lane < p.seqs.n_seqs) {
+            const RowRange r = kv8_rows(__ldg(p.seqs.row_start + s0 + lane), __ldg(p.seqs.row_start + s0 + lane + 1), p.seqs.rows);
+            blocks = ((r.r1 - r.r0) * p.group + ROWS - 1) / ROWS;
+        }
+        int sum = blocks;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, sum, o);
+            if (lane >= o) sum += v;
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, before + sum > want);
+        if (past) {
+            const int at = __ffs(past) - 1;
+            *status = fill_unit(p, s0 + at, tile, u);
+            u.head = index - want * H;
+            u.block = want - before - __shfl_sync(0xffffffffu, sum - blocks, at);
+            u.t0 = 0, u.t1 = u.tiles;
+            return u;
+        }
+        before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    return u;
+}
+
+// Where a CTA has a whole unit: its warps' sums, ROWS rows of D + 4 floats each (sums, R, l) at `part` +
+// warp * stride, to the output.
+template <int D, int WARPS>
+__device__ __forceinline__ void join_warps(const AttnKv8 &p, const Unit &u, int rows, const float *part, int stride) {
+    constexpr int E = D / 32;
+    const int lane = threadIdx.x & 31;
+    for (int r = threadIdx.x >> 5; r < rows; r += WARPS) {
+        const int x = u.block * p.tile_rows + r;
+        if (x >= u.n_rows) break;
+        const float ref = lane < WARPS ? part[lane * stride + r * (D + 4) + D] : -INFINITY;
+        float top = ref;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float f = top == -INFINITY ? 0.f : ex2(ref - top);
+        float l = lane < WARPS ? part[lane * stride + r * (D + 4) + D + 1] * f : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        float y[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) y[i] = 0.f;
+#pragma unroll 8
+        for (int w = 0; w < WARPS; ++w) {
+            const float fw = __shfl_sync(0xffffffffu, f, w);
+#pragma unroll
+            for (int i = 0; i < E; ++i) y[i] = fmaf(part[w * stride + r * (D + 4) + lane * E + i], fw, y[i]);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        store_row<E>(p, u.rr.r0 + x / p.group, u.head * p.group + x % p.group, lane * E, y, inv);
+    }
+}
+
+template <int D, int FORMAT, bool SPLIT, bool DIRECT>
 __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const __grid_constant__ AttnKv8 p) {
     using S = Ak8Shape<D>;
     constexpr int kRows = SPLIT ? 8 : 16;      // rows of a unit
     constexpr int NR = SPLIT ? 1 : 2;          // rows a lane holds
     constexpr int NJ = D / 8;                  // output columns a lane holds, per row: 2 NJ
-    constexpr int kGran = D / 16;              // granules of a row
+    constexpr int kChunks = D / 64;            // 64-wide chunks of a row
     extern __shared__ __align__(16) uint8_t smem[];
     uint32_t *plan = reinterpret_cast<uint32_t *>(smem + S::kRing);  // [n_seqs + 1]
-    __shared__ uint32_t warp_sum[S::kWarps];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int n_seqs = p.seqs.n_seqs, H = p.cache.kv_heads;
-
-    // ---- tiles before each sequence
-    {
-        uint32_t before = 0;
-        for (int s0 = 0; s0 < n_seqs; s0 += S::kWarps * 32) {
-            const int s = s0 + int(threadIdx.x);
-            uint32_t mine = 0;
-            if (s < n_seqs) {
-                const RowRange r = kv8_rows(__ldg(p.seqs.row_start + s), __ldg(p.seqs.row_start + s + 1), p.seqs.rows);
-                int status = 0;
-                if (r.r1 > r.r0) {
-                    const SeqSpan span = kv8_span(p.cache, __ldg(p.seqs.slot + s), __ldg(p.seqs.ctx_len + s), r.r1 - r.r0, &status);
-                    const uint32_t tiles = span.total > 0 ? (span.total + kAk8Tile - 1) / kAk8Tile : 1;
-                    mine = tiles * uint32_t(((r.r1 - r.r0) * p.group + kRows - 1) / kRows);
-                    if (blockIdx.x == 0) p.plan[n_seqs + 1 + s] = tiles;
-                }
-                if (blockIdx.x == 0) op_report(p.status, status);
-            }
-            uint32_t sum = mine;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-                if (lane >= o) sum += v;
-            }
-            if (lane == 31) warp_sum[warp] = sum;
-            __syncthreads();
-            uint32_t base = before, all = 0;
-            for (int w = 0; w < S::kWarps; ++w) {
-                if (w < warp) base += warp_sum[w];
-                all += warp_sum[w];
-            }
-            if (s < n_seqs) plan[s] = base + sum - mine;
-            before += all;
-            __syncthreads();
-        }
-        if (threadIdx.x == 0) plan[n_seqs] = before;
-        __syncthreads();
-        if (blockIdx.x == 0)
-            for (int s = threadIdx.x; s <= n_seqs; s += S::kWarps * 32) p.plan[s] = plan[s];
+    Run run{};
+    run.g_end = 1;
+    if (!DIRECT) {
+        const int64_t total = plan_tiles<kRows, kAk8Tile, S::kWarps>(p, plan);
+        if (!warp_run<S::kWarps>(p, total, run)) return;
     }
-    const int64_t total = int64_t(plan[n_seqs]) * H;
-    const int used = runs_used(total, p.workers);
-    const int worker = warp * gridDim.x + blockIdx.x;
-    if (worker >= used) return;
-    int64_t g = run_begin(total, used, worker);
-    const int64_t g_end = run_begin(total, used, worker + 1);
 
     uint8_t *ring = smem + warp * (S::kStage * S::kStages);
+    const int row8 = lane >> 2, t = lane & 3;  // the lane's row and column group in a product
     const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
-    const int row8 = lane >> 2, t = lane & 3;  // the lane's row and column pair in a product
 
-    while (g < g_end) {
-        // ---- which unit
-        int lo = 0, hi = n_seqs;  // the last sequence that begins at or before g and has tiles
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (int64_t(plan[mid]) * H <= g) lo = mid; else hi = mid;
-        }
-        const int s = lo;
-        const RowRange rr = kv8_rows(__ldg(p.seqs.row_start + s), __ldg(p.seqs.row_start + s + 1), p.seqs.rows);
-        const int slot = __ldg(p.seqs.slot + s);
+    while (run.g < run.g_end) {
         int status = 0;
-        const SeqSpan span = kv8_span(p.cache, slot, __ldg(p.seqs.ctx_len + s), rr.r1 - rr.r0, &status);
-        status = 0;  // reported above
-        const int tiles = span.total > 0 ? (span.total + kAk8Tile - 1) / kAk8Tile : 1;
-        const int64_t rem = g - int64_t(plan[s]) * H;
-        const int per_head = int(plan[s + 1] - plan[s]);
-        const int head = int(rem / per_head);
-        const int in_head = int(rem - int64_t(head) * per_head);
-        const int block = in_head / tiles;
-        const int t0 = in_head - block * tiles;
-        const int t1 = int(min(int64_t(tiles), t0 + (g_end - g)));
-        const int n_rows = (rr.r1 - rr.r0) * p.group;
-        const int32_t *table = p.cache.page_table + size_t(span.total > 0 ? slot : 0) * p.cache.pages_per_slot;
-        const int n_pages = (span.total + kKv8Page - 1) / kKv8Page;
+        const Unit u = DIRECT ? direct_unit<kRows>(p, blockIdx.x, kAk8Tile, &status) : find_unit(p, plan, run, kAk8Tile);
+        if (DIRECT && u.n_rows == 0) return;  // the whole CTA
+        const RowRange rr = u.rr;
+        const SeqSpan span = u.span;
+        const int head = u.head, block = u.block, t1 = u.t1, n_rows = u.n_rows;
+        const int t0 = u.t0 + (DIRECT ? warp : 0), step = DIRECT ? S::kWarps : 1;  // this warp's tiles
 
-        // ---- the copy of a tile into a stage; both pages' ids come one tile ahead
-        const auto page_ids = [&](int tile) {
-            int2 id = make_int2(-1, -1);
-            if (2 * tile < n_pages) id.x = kv8_page(p.cache, __ldg(table + 2 * tile), &status);
-            if (2 * tile + 1 < n_pages) id.y = kv8_page(p.cache, __ldg(table + 2 * tile + 1), &status);
-            return id;
+        // ---- the copies of a tile: lane i has the id of page i & 1, loaded a tile ahead of its use
+        const auto page_id = [&](int tile) {
+            const int i = 2 * tile + (lane & 1);
+            return tile < t1 && i < u.n_pages ? kv8_page(p.cache, __ldg(u.table + i), &status) : -1;
         };
-        const auto issue = [&](int tile, int stage, int2 id) {
-            const uint32_t dst = ring_s + uint32_t(stage * S::kStage);
-            const uint8_t *codes = static_cast<const uint8_t *>(p.cache.codes);
+        const auto issue = [&](int stage, int id) { copy_pages<D, 2>(p.cache, head, ring_s + stage * S::kStage, id); };
+        int ids[S::kStages];
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg) {
-                const int page = pg ? id.y : id.x;
-                const int left = page < 0 ? 0 : span.total - (2 * tile + pg) * kKv8Page;  // positions that exist
-                const size_t k_cell = kv8_cell(p.cache, page < 0 ? 0 : page, 0, head, 0);
-                const size_t v_cell = kv8_cell(p.cache, page < 0 ? 0 : page, 1, head, 0);
-#pragma unroll
-                for (int i = 0; i < kGran / 2; ++i) {
-                    const int at = i * 32 + lane, r = at / kGran;
-                    const uint32_t to = dst + uint32_t(pg * S::kBlock + granule<D>(r, at % kGran) * 16);
-                    const int bytes = r < left ? 16 : 0;  // what no position fills becomes zeros
-                    cp_async16(to, codes + k_cell * D + at * 16, bytes);
-                    cp_async16(to + 2 * S::kBlock, codes + v_cell * D + at * 16, bytes);
-                }
-                if (lane < 8) {
-                    const size_t cell = (lane < 4 ? k_cell : v_cell) + (lane & 3) * 4;
-                    cp_async16(dst + uint32_t(4 * S::kBlock + ((lane >> 2) * 2 + pg) * 64 + (lane & 3) * 16), p.cache.scales + cell,
-                               page < 0 ? 0 : 16);
-                }
-            }
-            cp_async_commit();
-        };
-
-        int2 ids[S::kStages];
-#pragma unroll
-        for (int i = 0; i < S::kStages; ++i) ids[i] = t0 + i < t1 ? page_ids(t0 + i) : make_int2(-1, -1);
+        for (int i = 0; i < S::kStages; ++i) ids[i] = page_id(t0 + i * step);
 #pragma unroll
         for (int i = 0; i < S::kStages - 1; ++i) {
-            if (t0 + i < t1) issue(t0 + i, i, ids[i]); else cp_async_commit();
+            if (t0 + i * step < t1) issue(i, ids[i]);
+            cp_async_commit();
         }
 
-        // ---- the query rows as fragments
+        // ---- the query rows as fragments; the sign of the scale goes into them
         uint32_t qf[D / 16][4];
-        float rf[NR];           // what a product's value has to be multiplied by
+        float rf[NR];           // what makes a product a score in log2, above 0
         int new_row[NR];        // which new row of the sequence; -1: none
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             const int x = block * kRows + row8 + r * 8;
-            float q[kGran / 4][2][8];
+            float q[kChunks][2][8];
             float top = 0.f;
             new_row[r] = x < n_rows ? x / p.group : -1;
             const int64_t at = int64_t(rr.r0 + x / p.group) * p.a.q_row_stride +
                                int64_t(head * p.group + x % p.group) * p.a.q_head_stride + t * 16;
 #pragma unroll
-            for (int c = 0; c < kGran / 4; ++c)
+            for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
                     if (new_row[r] >= 0) {
@@ -299,223 +433,231 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
-            const float to = pow2i(7 - e);
-            rf[r] = p.a.scale * 1.4426950408889634f * pow2i(e - 7);
+            const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
+            rf[r] = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
 #pragma unroll
-            for (int c = 0; c < kGran / 4; ++c)
+            for (int c = 0; c < kChunks; ++c)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const float *x4 = &q[c][j / 2][(j & 1) * 4];
                     if constexpr (SPLIT) {
-                        qf[c * 4 + j][0] = split2(x4[0] * to, x4[1] * to, &qf[c * 4 + j][1]);
-                        qf[c * 4 + j][2] = split2(x4[2] * to, x4[3] * to, &qf[c * 4 + j][3]);
+                        qf[c * 4 + j][0] = split2(make_float2(x4[0] * to, x4[1] * to), &qf[c * 4 + j][1]);
+                        qf[c * 4 + j][2] = split2(make_float2(x4[2] * to, x4[3] * to), &qf[c * 4 + j][3]);
                     } else {
-                        qf[c * 4 + j][r] = pack2(x4[0] * to, x4[1] * to);
-                        qf[c * 4 + j][2 + r] = pack2(x4[2] * to, x4[3] * to);
+                        qf[c * 4 + j][r] = pack2(make_float2(x4[0] * to, x4[1] * to));
+                        qf[c * 4 + j][2 + r] = pack2(make_float2(x4[2] * to, x4[3] * to));
                     }
                 }
         }
 
-        float o[NJ][2 * NR], m[NR], l[NR];
-        int E = 14;  // biased exponent of the largest V scale so far
+        float o[NJ][2 * NR], ref[NR], m[NR], l[NR];
+        int E = 40;  // biased exponent of the largest V scale so far (scales below 2^-87 lose bits of their weights)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int i = 0; i < 2 * NR; ++i) o[j][i] = 0.f;
 #pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = -INFINITY, l[r] = 0.f;
+        for (int r = 0; r < NR; ++r) m[r] = ref[r] = -INFINITY, l[r] = 0.f;
 
-        int2 id_now = ids[0], id_1 = ids[1], id_2 = S::kStages > 2 ? ids[S::kStages - 1] : make_int2(-1, -1);
         int stage = 0;
-        for (int tile = t0; tile < t1; ++tile) {
+        for (int tile = t0; tile < t1; tile += step) {
+            const int id_now = ids[0];
             {
-                const int ahead = tile + S::kStages - 1;
-                const int2 id = S::kStages > 2 ? id_2 : id_1;
                 int st = stage + S::kStages - 1;
                 if (st >= S::kStages) st -= S::kStages;
-                if (ahead < t1) issue(ahead, st, id); else cp_async_commit();
+                if (tile + (S::kStages - 1) * step < t1) issue(st, ids[S::kStages - 1]);
+                cp_async_commit();
+#pragma unroll
+                for (int i = 0; i < S::kStages - 1; ++i) ids[i] = ids[i + 1];
+                ids[S::kStages - 1] = page_id(tile + S::kStages * step);
             }
-            const int2 id_next = tile + S::kStages < t1 ? page_ids(tile + S::kStages) : make_int2(-1, -1);
             cp_async_wait<S::kStages - 1>();
             __syncwarp();
-            const uint8_t *st = ring + stage * S::kStage;
+            uint8_t *st = ring + stage * S::kStage;
             const float *sc = reinterpret_cast<const float *>(st + 4 * S::kBlock);  // [k, v][page][16]
-
-            // scores
-            float sv[2][2][2 * NR];  // [page][tau][row, e]
+            const int p0 = tile * kAk8Tile;
+            const uint32_t ok = __ballot_sync(0xffffffffu, id_now >= 0) & 3u;
+            // only tiles that reach into the new rows, or miss a page, have masks
+            const bool whole = p0 + kAk8Tile <= span.ctx && ok == 3u;
+            if (!whole) {  // V codes that no position fills become zeros: a weight of 0 has to stay 0
+                if (p0 + lane >= span.total || !(ok >> (lane >> 4) & 1u)) {
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg)
+                    for (int i = 0; i < D / 16; ++i)
+                        *reinterpret_cast<uint4 *>(st + 2 * S::kBlock + lane * D + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                __syncwarp();
+            }
+
+            // scores, without the rows' factors; pair i = (page, tau) holds two neighbouring positions
+            float2 sv[4][NR];
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg) {
+                const float4 ks = *reinterpret_cast<const float4 *>(sc + pg * 16 + 4 * t);
 #pragma unroll
                 for (int tau = 0; tau < 2; ++tau) {
-                    const int r = page_row(tau, row8 >> 1, row8 & 1);
-                    float c[4] = {0.f, 0.f, 0.f, 0.f};
+                    const int r = 4 * (row8 >> 1) + 2 * tau + (row8 & 1);
+                    float c[4];
 #pragma unroll
-                    for (int ch = 0; ch < kGran / 4; ++ch) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(st + pg * S::kBlock + granule<D>(r, ch * 4 + t) * 16);
+                    for (int ch = 0; ch < kChunks; ++ch) {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(st + pg * S::kBlock + r * D + ch * 64 + t * 16);
                         const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             uint32_t b0, b1;
                             codes_f16<FORMAT>(ww[j], b0, b1);
                             const uint32_t(&qa)[4] = qf[ch * 4 + j];
-                            mma16816(c, qa[0], qa[1], qa[2], qa[3], b0, b1);
+                            if (ch == 0 && j == 0)
+                                mma16816_0(c, qa[0], qa[1], qa[2], qa[3], b0, b1);
+                            else
+                                mma16816(c, qa[0], qa[1], qa[2], qa[3], b0, b1);
                         }
                     }
-                    const float k0 = sc[pg * 16 + page_row(tau, t, 0)], k1 = sc[pg * 16 + page_row(tau, t, 1)];
+                    const float2 k2 = tau ? make_float2(ks.z, ks.w) : make_float2(ks.x, ks.y);
                     if constexpr (SPLIT) {
-                        sv[pg][tau][0] = (c[0] + c[2]) * (k0 * rf[0]);
-                        sv[pg][tau][1] = (c[1] + c[3]) * (k1 * rf[0]);
+                        sv[pg * 2 + tau][0] = mul2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), k2);
                     } else {
-                        sv[pg][tau][0] = c[0] * (k0 * rf[0]);
-                        sv[pg][tau][1] = c[1] * (k1 * rf[0]);
-                        sv[pg][tau][2] = c[2] * (k0 * rf[1]);
-                        sv[pg][tau][3] = c[3] * (k1 * rf[1]);
+                        sv[pg * 2 + tau][0] = mul2(make_float2(c[0], c[1]), k2);
+                        sv[pg * 2 + tau][1] = mul2(make_float2(c[2], c[3]), k2);
                     }
                 }
-            // masks: only tiles that reach into the new rows, or miss a page, have any
-            const int p0 = tile * kAk8Tile;
-            const bool whole = p0 + kAk8Tile <= span.ctx && id_now.x >= 0 && id_now.y >= 0;
-            uint32_t seen[NR];  // bit (pg * 4 + tau * 2 + e)
-#pragma unroll
-            for (int r = 0; r < NR; ++r) seen[r] = 0xffu;
+            }
+            uint32_t seen[NR];  // bit: page * 4 + position within the lane's four
             if (!whole) {
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
                     seen[r] = 0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int pos = p0 + (i >> 2) * kKv8Page + page_row((i >> 1) & 1, t, i & 1);
-                        bool ok = pos < span.total && ((i >> 2) ? id_now.y : id_now.x) >= 0;
-                        const int j = pos - span.ctx;
-                        if (ok && j >= 0) {
+                        const int pos = p0 + (i >> 2) * kKv8Page + 4 * t + (i & 3), j = pos - span.ctx;
+                        bool in = pos < span.total && (ok >> (i >> 2) & 1u);
+                        if (in && j >= 0) {
                             if (new_row[r] < 0)
-                                ok = false;
+                                in = false;
                             else if (!p.a.mask)
-                                ok = j <= new_row[r];
+                                in = j <= new_row[r];
                             else
-                                ok = j < 32 * p.a.mask_words &&
+                                in = j < 32 * p.a.mask_words &&
                                      ((__ldg(p.a.mask + size_t(rr.r0 + new_row[r]) * p.a.mask_words + j / 32) >> (j & 31)) & 1u);
                         }
-                        seen[r] |= ok ? 1u << i : 0u;
+                        seen[r] |= in ? 1u << i : 0u;
+                        if (!in) ((i & 1) ? sv[i >> 1][r].y : sv[i >> 1][r].x) = -INFINITY;
                     }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i)
-                        if (!(seen[r] >> i & 1u)) {
-                            sv[i >> 2][(i >> 1) & 1][2 * r + (i & 1)] = -INFINITY;
-                        }
                 }
             }
             // the running exponent of the V scales
-            int E_new;
             {
-                const int pos = p0 + lane;
-                uint32_t b = 0;
-                if (pos < span.total) b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
-                if (b >= 0x7f800000u) b = 0;
-                E_new = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+                uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
+                if (b >= 0x7f800000u || p0 + lane >= span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
+                E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
             }
-            const float v_to = pow2i(140 - E_new), v_fix = E_new - E > 126 ? 0.f : pow2i(E - E_new);
-            E = E_new;
             // softmax
             float corr[NR];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) mx = fmaxf(mx, sv[i >> 2][(i >> 1) & 1][2 * r + (i & 1)]);
+                float mx = fmaxf(fmaxf(fmaxf(sv[0][r].x, sv[0][r].y), fmaxf(sv[1][r].x, sv[1][r].y)),
+                                 fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                 mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                const float m_new = fmaxf(m[r], mx);
-                const float ref = m_new == -INFINITY ? 0.f : m_new;
-                corr[r] = exp2_approx(m[r] - ref);
-                m[r] = m_new;
-                float sum = 0.f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float &x = sv[i >> 2][(i >> 1) & 1][2 * r + (i & 1)];
-                    x = exp2_approx(x - ref);
-                    sum += x;
-                }
-                l[r] = fmaf(l[r], corr[r], sum);
-                corr[r] *= v_fix;
-            }
-            if constexpr (!SPLIT) {
-                // the sums stay in the products' accumulators
-#pragma unroll
-                for (int j = 0; j < NJ; ++j) {
-                    o[j][0] *= corr[0], o[j][1] *= corr[0];
-                    o[j][2] *= corr[1], o[j][3] *= corr[1];
-                }
-            }
-#pragma unroll
-            for (int pg = 0; pg < 2; ++pg) {
-                uint32_t wa[4];  // the weights as the left operand: tau 0 rows g, g + 8, tau 1 rows g, g + 8
-#pragma unroll
-                for (int tau = 0; tau < 2; ++tau) {
-                    const float v0 = sc[32 + pg * 16 + page_row(tau, t, 0)] * v_to, v1 = sc[32 + pg * 16 + page_row(tau, t, 1)] * v_to;
-                    const int bit = pg * 4 + tau * 2;
-                    // a masked position's scale may be anything, NaN included
-                    const auto weight = [&](int r, int e, float v) {
-                        return (seen[r] >> (bit + e) & 1u) ? sv[pg][tau][2 * r + e] * v : 0.f;
-                    };
-                    if constexpr (SPLIT) {
-                        wa[tau * 2] = split2(weight(0, 0, v0), weight(0, 1, v1), &wa[tau * 2 + 1]);
-                    } else {
-                        wa[tau * 2] = pack2(weight(0, 0, v0), weight(0, 1, v1));
-                        wa[tau * 2 + 1] = pack2(weight(1, 0, v0), weight(1, 1, v1));
-                    }
-                }
-                uint32_t vw[4][D / 32];  // [2 tau + e][word]
+                m[r] = fmaxf(m[r], mx * rf[r]);
+                const float now = m[r] == -INFINITY ? -INFINITY : m[r] - float(140 - E);
+                const float use = now == -INFINITY ? 0.f : now;
+                corr[r] = ex2(ref[r] - use);
+                ref[r] = now;
+                const float2 rf2 = make_float2(rf[r], rf[r]), off = make_float2(-use, -use);
+                float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int r = page_row(i >> 1, t, i & 1);
-                    const uint8_t *src = st + 2 * S::kBlock + pg * S::kBlock;
-                    if constexpr (D == 64) {
-                        const uint2 w = *reinterpret_cast<const uint2 *>(src + granule<D>(r, row8 >> 1) * 16 + (row8 & 1) * 8);
-                        vw[i][0] = w.x, vw[i][1] = w.y;
+                    float2 &x = sv[i][r];
+                    x = fma2(x, rf2, off);
+                    x.x = ex2(x.x), x.y = ex2(x.y);
+                    sum = add2(sum, x);
+                }
+                l[r] = fmaf(l[r], corr[r], sum.x + sum.y);
+            }
+            // weights as the left operand: tau 0 rows g, g + 8, tau 1 rows g, g + 8
+            uint32_t wa[2][4];
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg) {
+                const float4 vs = *reinterpret_cast<const float4 *>(sc + 32 + pg * 16 + 4 * t);
+#pragma unroll
+                for (int tau = 0; tau < 2; ++tau) {
+                    const float2 v2 = tau ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y);
+                    float2 w[NR];
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        w[r] = mul2(sv[pg * 2 + tau][r], v2);
+                        if (!whole) {  // a masked position's scale may be anything, NaN included
+                            if (!(seen[r] >> (pg * 4 + tau * 2) & 1u)) w[r].x = 0.f;
+                            if (!(seen[r] >> (pg * 4 + tau * 2 + 1) & 1u)) w[r].y = 0.f;
+                        }
+                    }
+                    if constexpr (SPLIT) {
+                        wa[pg][tau * 2] = split2(w[0], &wa[pg][tau * 2 + 1]);
                     } else {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(src + granule<D>(r, row8) * 16);
-                        vw[i][0] = w.x, vw[i][1] = w.y, vw[i][2] = w.z, vw[i][3] = w.w;
+                        wa[pg][tau * 2] = pack2(w[0]);
+                        wa[pg][tau * 2 + 1] = pack2(w[1]);
+                    }
+                }
+            }
+            if constexpr (!SPLIT) {
+                // the sums stay in the products' accumulators; most tiles raise no maximum
+                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+#pragma unroll
+                    for (int j = 0; j < NJ; ++j) {
+                        o[j][0] *= corr[0], o[j][1] *= corr[0];
+                        o[j][2] *= corr[1], o[j][3] *= corr[1];
+                    }
+                }
+            }
+            uint32_t vw[2][4][D / 32];  // [page][position][word]
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const uint8_t *from = st + (2 + pg) * S::kBlock + (4 * t + i) * D + row8 * (D / 8);
+                    if constexpr (D == 64) {
+                        const uint2 w = *reinterpret_cast<const uint2 *>(from);
+                        vw[pg][i][0] = w.x, vw[pg][i][1] = w.y;
+                    } else {
+                        const uint4 w = *reinterpret_cast<const uint4 *>(from);
+                        vw[pg][i][0] = w.x, vw[pg][i][1] = w.y, vw[pg][i][2] = w.z, vw[pg][i][3] = w.w;
                     }
                 }
 #pragma unroll
-                for (int w = 0; w < D / 32; ++w)
+            for (int w = 0; w < D / 32; ++w)
 #pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        uint32_t b0[2], b1[2];  // of columns 4 w + 2 half and the next
-                        codes_f16<FORMAT>(__byte_perm(vw[0][w], vw[1][w], half ? 0x7362 : 0x5140), b0[0], b0[1]);
-                        codes_f16<FORMAT>(__byte_perm(vw[2][w], vw[3][w], half ? 0x7362 : 0x5140), b1[0], b1[1]);
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t b0[2][2], b1[2][2];  // [page], of columns 4 w + 2 half and the next
 #pragma unroll
-                        for (int k = 0; k < 2; ++k) {
-                            float(&oj)[2 * NR] = o[4 * w + 2 * half + k];
-                            if constexpr (SPLIT) {
-                                float c[4] = {0.f, 0.f, 0.f, 0.f};
-                                mma16816(c, wa[0], wa[1], wa[2], wa[3], b0[k], b1[k]);
-                                oj[0] = (pg == 0 ? oj[0] * corr[0] : oj[0]) + (c[0] + c[2]);
-                                oj[1] = (pg == 0 ? oj[1] * corr[0] : oj[1]) + (c[1] + c[3]);
-                            } else {
-                                mma16816(oj, wa[0], wa[1], wa[2], wa[3], b0[k], b1[k]);
-                            }
+                    for (int pg = 0; pg < 2; ++pg) {
+                        codes_f16<FORMAT>(__byte_perm(vw[pg][0][w], vw[pg][1][w], half ? 0x7362 : 0x5140), b0[pg][0], b0[pg][1]);
+                        codes_f16<FORMAT>(__byte_perm(vw[pg][2][w], vw[pg][3][w], half ? 0x7362 : 0x5140), b1[pg][0], b1[pg][1]);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        float(&oj)[2 * NR] = o[4 * w + 2 * half + k];
+                        if constexpr (SPLIT) {
+                            float c[4];
+                            mma16816_0(c, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b0[0][k], b1[0][k]);
+                            mma16816(c, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b0[1][k], b1[1][k]);
+                            const float2 y = fma2(make_float2(oj[0], oj[1]), make_float2(corr[0], corr[0]),
+                                                  add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                            oj[0] = y.x, oj[1] = y.y;
+                        } else {
+                            mma16816(oj, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b0[0][k], b1[0][k]);
+                            mma16816(oj, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b0[1][k], b1[1][k]);
                         }
                     }
-            }
+                }
             __syncwarp();  // the stage is free again
-            id_now = id_1;
-            if constexpr (S::kStages > 2) {
-                id_1 = id_2;
-                id_2 = id_next;
-            } else {
-                id_1 = id_next;
-            }
             if (++stage == S::kStages) stage = 0;
         }
-        cp_async_wait<0>();
-        __syncwarp();
         op_report(p.status, status);
 
-        // ---- results: lane (g, t) has of its rows the elements 16 t NJ/8 .. in two runs of NJ
-        const bool all = t0 == 0 && t1 == tiles;
-        const float v_back = pow2i(max(-126, E - 140));
+        // ---- results: lane (g, t) has of its rows the elements 2 NJ t .. in two runs of NJ
+        const bool all = !DIRECT && u.t0 == 0 && t1 == u.tiles;
+        float *part = DIRECT ? reinterpret_cast<float *>(ring) : p.part + size_t(2 * run.item + (u.t0 == 0 ? 1 : 0)) * p.part_rows * (D + 4);
+        if (DIRECT) __syncwarp();  // the ring is read no more
 #pragma unroll
         for (int r = 0; r < NR; ++r) {
             l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
@@ -523,7 +665,7 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
             if (new_row[r] < 0) continue;
             const int x = block * kRows + row8 + r * 8;
             if (all) {
-                const float f = l[r] == 0.f ? 0.f : v_back / l[r];
+                const float f = l[r] == 0.f ? 0.f : 1.f / l[r];
                 const int64_t at = int64_t(rr.r0 + new_row[r]) * p.a.out_row_stride +
                                    int64_t(head * p.group + x % p.group) * p.a.out_head_stride + t * (2 * NJ);
 #pragma unroll
@@ -536,18 +678,302 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
                         store_out8(p.a.out, p.a.type, p.vec_out != 0, at + e * NJ + j, y);
                     }
             } else {
-                float *part = p.part + (size_t(2 * worker + (t0 == 0 ? 1 : 0)) * p.part_rows + (row8 + r * 8)) * (D + 4);
+                float *to = part + (row8 + r * 8) * (D + 4);
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int j = 0; j < NJ; j += 4)
-                        *reinterpret_cast<float4 *>(part + t * (2 * NJ) + e * NJ + j) =
-                            make_float4(o[j][2 * r + e] * v_back, o[j + 1][2 * r + e] * v_back, o[j + 2][2 * r + e] * v_back,
-                                        o[j + 3][2 * r + e] * v_back);
-                if (t == 0) part[D] = m[r], part[D + 1] = l[r];
+                        *reinterpret_cast<float4 *>(to + t * (2 * NJ) + e * NJ + j) =
+                            make_float4(o[j][2 * r + e], o[j + 1][2 * r + e], o[j + 2][2 * r + e], o[j + 3][2 * r + e]);
+                if (t == 0) to[D] = ref[r], to[D + 1] = l[r];
             }
         }
-        g += t1 - t0;
+        if (DIRECT) {
+            __syncthreads();
+            join_warps<D, S::kWarps>(p, u, kRows, reinterpret_cast<const float *>(smem), S::kStage * S::kStages / 4);
+            return;
+        }
+        run.g += t1 - t0;
+    }
+}
+
+// The same for up to 4 query rows a unit (one new token of up to 4 heads a kv head): the products
+// are turned over, K and V^T on the left (16 positions, 16 columns of V) and the rows, split into
+// upper and lower parts, as the 8 columns on the right.  That takes half the products of the form
+// above and leaves lane (g, t) with row t's scores of positions g' and g' + 8, g' = (g >> 1) + 4 (g & 1),
+// of a page, so that four rows' softmax occupies every lane; movmatrix turns the weights into the
+// right operand of w V.
+template <int D, int FORMAT, bool DIRECT>
+__global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(const __grid_constant__ AttnKv8 p) {
+    using S = Ak8Few<D>;
+    constexpr int NP = S::kPages, kTile = NP * kKv8Page;
+    constexpr int NO = D / 8;                  // output columns a lane holds
+    constexpr int kChunks = D / 64;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint32_t *plan = reinterpret_cast<uint32_t *>(smem + S::kRing);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    Run run{};
+    run.g_end = 1;
+    if (!DIRECT) {
+        const int64_t total = plan_tiles<4, kTile, S::kWarps>(p, plan);
+        if (!warp_run<S::kWarps>(p, total, run)) return;
+    }
+
+    uint8_t *ring = smem + warp * (S::kStage * S::kStages);
+    const int row8 = lane >> 2, t = lane & 3;
+    const int mine = (row8 >> 1) + 4 * (row8 & 1);  // the lane's first position in a page; the second is 8 on
+    const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
+
+    while (run.g < run.g_end) {
+        int status = 0;
+        const Unit u = DIRECT ? direct_unit<4>(p, blockIdx.x, kTile, &status) : find_unit(p, plan, run, kTile);
+        if (DIRECT && u.n_rows == 0) return;  // the whole CTA
+        const int t1 = u.t1, t0 = u.t0 + (DIRECT ? warp : 0), step = DIRECT ? S::kWarps : 1;  // this warp's tiles
+
+        // ---- the copies of a tile: lane i has the id of page i % NP, loaded a tile ahead of its use
+        const auto page_id = [&](int tile) {
+            const int i = NP * tile + (lane & (NP - 1));
+            return tile < t1 && i < u.n_pages ? kv8_page(p.cache, __ldg(u.table + i), &status) : -1;
+        };
+        const auto issue = [&](int stage, int id) { copy_pages<D, NP>(p.cache, u.head, ring_s + stage * S::kStage, id); };
+        int ids[S::kStages];
+#pragma unroll
+        for (int i = 0; i < S::kStages; ++i) ids[i] = page_id(t0 + i * step);
+#pragma unroll
+        for (int i = 0; i < S::kStages - 1; ++i) {
+            if (t0 + i * step < t1) issue(i, ids[i]);
+            cp_async_commit();
+        }
+
+        // ---- the query: column g of the right operand is row g >> 1, upper part for even g, lower for odd
+        uint32_t qf[D / 16][2];
+        float rf;               // of row t
+        {
+            const int x = u.block * 4 + (row8 >> 1);
+            float q[kChunks][2][8];
+            float top = 0.f;
+            const int64_t at = int64_t(u.rr.r0 + x / p.group) * p.a.q_row_stride +
+                               int64_t(u.head * p.group + x % p.group) * p.a.q_head_stride + t * 16;
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    if (x < u.n_rows) {
+                        load_q8(p.a.q, p.a.type, p.vec_q != 0, at + c * 64 + hf * 8, q[c][hf]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) q[c][hf][i] = 0.f;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[c][hf][i]));
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
+            const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
+            rf = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
+            rf = __shfl_sync(0xffffffffu, rf, t * 8);
+#pragma unroll
+            for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float *x4 = &q[c][j / 2][(j & 1) * 4];
+                    uint32_t low[2];
+                    qf[c * 4 + j][0] = split2(make_float2(x4[0] * to, x4[1] * to), &low[0]);
+                    qf[c * 4 + j][1] = split2(make_float2(x4[2] * to, x4[3] * to), &low[1]);
+                    if (row8 & 1) qf[c * 4 + j][0] = low[0], qf[c * 4 + j][1] = low[1];
+                }
+        }
+        const int x_row = u.block * 4 + t;
+        const int new_row = x_row < u.n_rows ? x_row / p.group : -1;
+
+        float o[NO], ref = -INFINITY, m = -INFINITY, l = 0.f;
+        int E = 40;
+#pragma unroll
+        for (int j = 0; j < NO; ++j) o[j] = 0.f;
+
+        int stage = 0;
+        for (int tile = t0; tile < t1; tile += step) {
+            const int id_now = ids[0];
+            {
+                int st = stage + S::kStages - 1;
+                if (st >= S::kStages) st -= S::kStages;
+                if (tile + (S::kStages - 1) * step < t1) issue(st, ids[S::kStages - 1]);
+                cp_async_commit();
+#pragma unroll
+                for (int i = 0; i < S::kStages - 1; ++i) ids[i] = ids[i + 1];
+                ids[S::kStages - 1] = page_id(tile + S::kStages * step);
+            }
+            cp_async_wait<S::kStages - 1>();
+            __syncwarp();
+            uint8_t *st = ring + stage * S::kStage;
+            const float *sc = reinterpret_cast<const float *>(st + 2 * NP * S::kBlock);  // [k, v][page][16]
+            const int p0 = tile * kTile;
+            const uint32_t ok = __ballot_sync(0xffffffffu, id_now >= 0) & ((1u << NP) - 1);
+            const bool whole = p0 + kTile <= u.span.ctx && ok == (1u << NP) - 1;
+            if (!whole) {  // V codes that no position fills become zeros: a weight of 0 has to stay 0
+#pragma unroll
+                for (int k = 0; k < NP / 2; ++k) {
+                    const int r = lane + 32 * k;
+                    if (p0 + r >= u.span.total || !(ok >> (r >> 4) & 1u)) {
+#pragma unroll
+                        for (int i = 0; i < D / 16; ++i)
+                            *reinterpret_cast<uint4 *>(st + NP * S::kBlock + r * D + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    }
+                }
+                __syncwarp();
+            }
+
+            // scores of row t, without its factor
+            float2 sv[NP];
+#pragma unroll
+            for (int pg = 0; pg < NP; ++pg) {
+                float c[4];
+#pragma unroll
+                for (int ch = 0; ch < kChunks; ++ch) {
+                    const uint8_t *from = st + pg * S::kBlock + mine * D + ch * 64 + t * 16;
+                    const uint4 w0 = *reinterpret_cast<const uint4 *>(from), w1 = *reinterpret_cast<const uint4 *>(from + 8 * D);
+                    const uint32_t a_w[4] = {w0.x, w0.y, w0.z, w0.w}, b_w[4] = {w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        uint32_t a0, a1, a2, a3;
+                        codes_f16<FORMAT>(a_w[j], a0, a2);
+                        codes_f16<FORMAT>(b_w[j], a1, a3);
+                        if (ch == 0 && j == 0)
+                            mma16816_0(c, a0, a1, a2, a3, qf[0][0], qf[0][1]);
+                        else
+                            mma16816(c, a0, a1, a2, a3, qf[ch * 4 + j][0], qf[ch * 4 + j][1]);
+                    }
+                }
+                sv[pg] = mul2(make_float2(c[0] + c[1], c[2] + c[3]), make_float2(sc[pg * 16 + mine], sc[pg * 16 + mine + 8]));
+            }
+            uint32_t seen = 0;  // bit: 2 page + (0 or 1)
+            if (!whole) {
+#pragma unroll
+                for (int i = 0; i < 2 * NP; ++i) {
+                    const int pos = p0 + (i >> 1) * kKv8Page + mine + 8 * (i & 1), j = pos - u.span.ctx;
+                    bool in = pos < u.span.total && (ok >> (i >> 1) & 1u);
+                    if (in && j >= 0) {
+                        if (new_row < 0)
+                            in = false;
+                        else if (!p.a.mask)
+                            in = j <= new_row;
+                        else
+                            in = j < 32 * p.a.mask_words &&
+                                 ((__ldg(p.a.mask + size_t(u.rr.r0 + new_row) * p.a.mask_words + j / 32) >> (j & 31)) & 1u);
+                    }
+                    seen |= in ? 1u << i : 0u;
+                    if (!in) ((i & 1) ? sv[i >> 1].y : sv[i >> 1].x) = -INFINITY;
+                }
+            }
+            // the running exponent of the V scales
+            {
+                uint32_t b = 0;
+#pragma unroll
+                for (int k = 0; k < NP / 2; ++k) {
+                    const int r = lane + 32 * k;
+                    uint32_t v = __float_as_uint(sc[NP * 16 + r]) & 0x7fffffffu;
+                    if (v >= 0x7f800000u || (!whole && (p0 + r >= u.span.total || !(ok >> (r >> 4) & 1u)))) v = 0;
+                    b = max(b, v);
+                }
+                E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+            }
+            // softmax over the lanes of equal t
+            float mx = fmaxf(sv[0].x, sv[0].y);
+#pragma unroll
+            for (int i = 1; i < NP; ++i) mx = fmaxf(mx, fmaxf(sv[i].x, sv[i].y));
+#pragma unroll
+            for (int i = 4; i < 32; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
+            m = fmaxf(m, mx * rf);
+            const float now = m == -INFINITY ? -INFINITY : m - float(140 - E);
+            const float use = now == -INFINITY ? 0.f : now;
+            const float corr = ex2(ref - use);
+            ref = now;
+            const float2 rf2 = make_float2(rf, rf), off = make_float2(-use, -use);
+            float2 sum = make_float2(0.f, 0.f);
+            uint32_t wb[NP][2];  // weights as the right operand
+#pragma unroll
+            for (int pg = 0; pg < NP; ++pg) {
+                float2 x = fma2(sv[pg], rf2, off);
+                x.x = ex2(x.x), x.y = ex2(x.y);
+                sum = add2(sum, x);
+                float2 w = mul2(x, make_float2(sc[NP * 16 + pg * 16 + mine], sc[NP * 16 + pg * 16 + mine + 8]));
+                if (!whole) {  // a masked position's scale may be anything, NaN included
+                    if (!(seen >> (2 * pg) & 1u)) w.x = 0.f;
+                    if (!(seen >> (2 * pg + 1) & 1u)) w.y = 0.f;
+                }
+                // (upper, lower) of each of the two positions, then row t to column 2 t and 2 t + 1
+                const float2 up = __half22float2(__float22half2_rn(w));
+                const uint32_t first = pack2(make_float2(up.x, w.x - up.x)), second = pack2(make_float2(up.y, w.y - up.y));
+                asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(wb[pg][0]) : "r"(first));
+                asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(wb[pg][1]) : "r"(second));
+            }
+            l = fmaf(l, corr, sum.x + sum.y);
+            // w V: positions t, t + 4 (k = 2 t, 2 t + 1) and t + 8, t + 12 (k + 8) of a page
+#pragma unroll
+            for (int wp = 0; wp < D / 64; ++wp) {
+                uint2 vw[NP][4];
+#pragma unroll
+                for (int pg = 0; pg < NP; ++pg)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        vw[pg][i] = *reinterpret_cast<const uint2 *>(st + (NP + pg) * S::kBlock + (t + 4 * i) * D + row8 * (D / 8) + wp * 8);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {  // columns 8 wp + 2 k, + 1 of the lane's
+                    float c[4];
+#pragma unroll
+                    for (int pg = 0; pg < NP; ++pg) {
+                        const uint32_t sel = k & 1 ? 0x7362 : 0x5140;
+                        uint32_t a0, a1, a2, a3;
+                        codes_f16<FORMAT>(__byte_perm(k < 2 ? vw[pg][0].x : vw[pg][0].y, k < 2 ? vw[pg][1].x : vw[pg][1].y, sel), a0, a1);
+                        codes_f16<FORMAT>(__byte_perm(k < 2 ? vw[pg][2].x : vw[pg][2].y, k < 2 ? vw[pg][3].x : vw[pg][3].y, sel), a2, a3);
+                        if (pg == 0)
+                            mma16816_0(c, a0, a1, a2, a3, wb[0][0], wb[0][1]);
+                        else
+                            mma16816(c, a0, a1, a2, a3, wb[pg][0], wb[pg][1]);
+                    }
+                    o[wp * 8 + 2 * k] = fmaf(o[wp * 8 + 2 * k], corr, c[0] + c[1]);
+                    o[wp * 8 + 2 * k + 1] = fmaf(o[wp * 8 + 2 * k + 1], corr, c[2] + c[3]);
+                }
+            }
+            __syncwarp();  // the stage is free again
+            if (++stage == S::kStages) stage = 0;
+        }
+        op_report(p.status, status);
+
+        // ---- results: lane (g, t) has columns NO g .. of row t
+#pragma unroll
+        for (int i = 4; i < 32; i <<= 1) l += __shfl_xor_sync(0xffffffffu, l, i);
+        float *part = DIRECT ? reinterpret_cast<float *>(ring) : p.part + size_t(2 * run.item + (u.t0 == 0 ? 1 : 0)) * p.part_rows * (D + 4);
+        if (DIRECT) __syncwarp();  // the ring is read no more
+        if (new_row >= 0) {
+            if (!DIRECT && u.t0 == 0 && t1 == u.tiles) {
+                const float f = l == 0.f ? 0.f : 1.f / l;
+                const int64_t at = int64_t(u.rr.r0 + new_row) * p.a.out_row_stride +
+                                   int64_t(u.head * p.group + x_row % p.group) * p.a.out_head_stride + row8 * NO;
+#pragma unroll
+                for (int j = 0; j < NO; j += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = o[j + i] * f;
+                    store_out8(p.a.out, p.a.type, p.vec_out != 0, at + j, y);
+                }
+            } else {
+                float *to = part + t * (D + 4);
+#pragma unroll
+                for (int j = 0; j < NO; j += 4)
+                    *reinterpret_cast<float4 *>(to + row8 * NO + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                if (row8 == 0) to[D] = ref, to[D + 1] = l;
+            }
+        }
+        if (DIRECT) {
+            __syncthreads();
+            join_warps<D, S::kWarps>(p, u, 4, reinterpret_cast<const float *>(smem), S::kStage * S::kStages / 4);
+            return;
+        }
+        run.g += t1 - t0;
     }
 }
 
@@ -566,13 +992,13 @@ __global__ void __launch_bounds__(256) k_attn_kv8_join(const __grid_constant__ A
     if (row >= rr.r1) return;
     const int H = p.cache.kv_heads, head = qh / p.group;
     const int x = (row - rr.r0) * p.group + (qh - head * p.group), block = x / p.tile_rows;
-    const uint32_t before = __ldcg(p.plan + s), after = __ldcg(p.plan + s + 1), tiles = __ldcg(p.plan + p.seqs.n_seqs + 1 + s);
-    const int64_t total = int64_t(__ldcg(p.plan + p.seqs.n_seqs)) * H;
-    const int used = runs_used(total, p.workers);
-    const int64_t g0 = int64_t(before) * H + int64_t(head) * (after - before) + int64_t(block) * tiles, g1 = g0 + tiles;
+    const uint32_t before = __ldcg(p.plan + s), tiles = __ldcg(p.plan + p.seqs.n_seqs + 1 + s);
+    const int64_t total = __ldcg(p.plan + p.seqs.n_seqs);
+    const int used = runs_used(total, p.runs);
+    const int64_t g0 = int64_t(before) + int64_t(block) * tiles, g1 = g0 + tiles;
     const int w0 = run_of(total, used, g0), w1 = run_of(total, used, g1 - 1);
     if (w0 == w1) return;  // written whole
-    // worker w0 begins the unit at its run's second place unless the run itself begins here
+    // run w0 begins the unit, the others begin inside it
     constexpr int E = D / 32;
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
@@ -581,7 +1007,7 @@ __global__ void __launch_bounds__(256) k_attn_kv8_join(const __grid_constant__ A
     const size_t slot = size_t(p.part_rows) * (D + 4);
 #pragma unroll 4
     for (int w = w0; w <= w1; ++w) {
-        const float *part = p.part + size_t(2 * w + (w == w0 ? 1 : 0)) * slot + in_slot;
+        const float *part = p.part + (size_t(w) * H + head) * 2 * slot + (w == w0 ? slot : 0) + in_slot;
         float v[E];
         if constexpr (E == 2) {
             const float2 a = __ldcg(reinterpret_cast<const float2 *>(part) + lane);
@@ -592,24 +1018,14 @@ __global__ void __launch_bounds__(256) k_attn_kv8_join(const __grid_constant__ A
         }
         const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part + D));
         const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float fa = exp2_approx(m - ref), fb = exp2_approx(ml.x - ref);
+        const float fa = ex2(m - ref), fb = ex2(ml.x - ref);
         m = m_new;
         l = l * fa + ml.y * fb;
 #pragma unroll
         for (int i = 0; i < E; ++i) o[i] = o[i] * fa + v[i] * fb;
     }
     const float f = l == 0.f ? 0.f : 1.f / l;
-    const int64_t at = int64_t(row) * p.a.out_row_stride + int64_t(qh) * p.a.out_head_stride + lane * E;
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-        const float y = o[i] * f;
-        if (p.a.type == MOSSGPU_F32)
-            static_cast<float *>(p.a.out)[at + i] = y;
-        else if (p.a.type == MOSSGPU_F16)
-            static_cast<__half *>(p.a.out)[at + i] = __float2half_rn(y);
-        else
-            static_cast<__nv_bfloat16 *>(p.a.out)[at + i] = __float2bfloat16_rn(y);
-    }
+    store_row<E>(p, row, qh, lane * E, o, f);
 }
 
 }  // namespace mossgpu

@@ -29,7 +29,7 @@ int check_cache(const mossgpu_kv8_cache *c, const char *who) {
     if (c->n_pages < 1 || c->n_slots < 1 || c->pages_per_slot < 1)
         return op_errorf("%s: n_pages, n_slots and pages_per_slot must be positive", who);
     if (c->pages_per_slot > (1 << 26)) return op_errorf("%s: pages_per_slot is above 2^26", who);
-    if (c->kv_heads < 1 || c->kv_heads > 4096) return op_errorf("%s: kv_heads = %d must be 1 .. 4096", who, c->kv_heads);
+    if (c->kv_heads < 1 || c->kv_heads > 1024) return op_errorf("%s: kv_heads = %d must be 1 .. 1024", who, c->kv_heads);
     if (c->head_dim != 64 && c->head_dim != 128) return op_errorf("%s: head_dim = %d must be 64 or 128", who, c->head_dim);
     if (c->format != MOSSGPU_KV_INT8 && c->format != MOSSGPU_KV_E4M3) return op_errorf("%s: format %d is none", who, c->format);
     return 0;
@@ -109,29 +109,38 @@ cudaError_t launch_read(ReadOp a, cudaStream_t st) {
 
 // ---- attention ---------------------------------------------------------------------------
 
-// rows of a unit: 8 where the products are split into upper and lower parts, else 16
-int unit_rows(int type) { return type == MOSSGPU_BF16 ? 16 : 8; }
-int warps_of(int head_dim) { return head_dim == 64 ? Ak8Shape<64>::kWarps : Ak8Shape<128>::kWarps; }
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 size_t plan_bytes() { return round256(sizeof(uint32_t) * (2 * kAk8MaxSeqs + 1)); }
 
+// The kernel of a call: which form, and what it needs.
+struct AttnForm {
+    void (*kernel)(AttnKv8), (*direct)(AttnKv8);
+    int warps, ring, tile_rows;
+};
+
+template <int D, int FORMAT>
+AttnForm attn_form(int type, int64_t rows_per_unit) {
+    if (rows_per_unit <= 4)
+        return {k_attn_kv8_few<D, FORMAT, false>, k_attn_kv8_few<D, FORMAT, true>, Ak8Few<D>::kWarps, Ak8Few<D>::kRing, 4};
+    using S = Ak8Shape<D>;
+    if (type == MOSSGPU_BF16) return {k_attn_kv8<D, FORMAT, false, false>, k_attn_kv8<D, FORMAT, false, true>, S::kWarps, S::kRing, 16};
+    return {k_attn_kv8<D, FORMAT, true, false>, k_attn_kv8<D, FORMAT, true, true>, S::kWarps, S::kRing, 8};
+}
+
+// Mean query rows of a sequence and kv head decide: the forms differ in speed, not in what they can do.
+AttnForm attn_form(int head_dim, int format, int type, int64_t rows, int n_seqs, int group) {
+    const int64_t per_unit = (rows + n_seqs - 1) / n_seqs * group;
+    if (head_dim == 64)
+        return format == MOSSGPU_KV_INT8 ? attn_form<64, MOSSGPU_KV_INT8>(type, per_unit) : attn_form<64, MOSSGPU_KV_E4M3>(type, per_unit);
+    return format == MOSSGPU_KV_INT8 ? attn_form<128, MOSSGPU_KV_INT8>(type, per_unit) : attn_form<128, MOSSGPU_KV_E4M3>(type, per_unit);
+}
+
+// Enough for every form
 size_t workspace_of(int head_dim, int64_t rows_in_unit) {
-    const size_t part = std::min<int64_t>(16, rows_in_unit) * size_t(head_dim + 4) * sizeof(float);
-    return plan_bytes() + size_t(2) * kNumSMs * warps_of(head_dim) * part;
-}
-
-using AttnKernel = void (*)(AttnKv8);
-AttnKernel attn_kernel(int head_dim, int format, bool split) {
-    if (head_dim == 64) {
-        if (format == MOSSGPU_KV_INT8) return split ? k_attn_kv8<64, MOSSGPU_KV_INT8, true> : k_attn_kv8<64, MOSSGPU_KV_INT8, false>;
-        return split ? k_attn_kv8<64, MOSSGPU_KV_E4M3, true> : k_attn_kv8<64, MOSSGPU_KV_E4M3, false>;
-    }
-    if (format == MOSSGPU_KV_INT8) return split ? k_attn_kv8<128, MOSSGPU_KV_INT8, true> : k_attn_kv8<128, MOSSGPU_KV_INT8, false>;
-    return split ? k_attn_kv8<128, MOSSGPU_KV_E4M3, true> : k_attn_kv8<128, MOSSGPU_KV_E4M3, false>;
-}
-
-int attn_smem(int head_dim, int n_seqs) {
-    return (head_dim == 64 ? Ak8Shape<64>::kRing : Ak8Shape<128>::kRing) + int(sizeof(uint32_t)) * (n_seqs + 1);
+    const size_t row = size_t(head_dim + 4) * sizeof(float);
+    const int few = head_dim == 64 ? Ak8Few<64>::kWarps : Ak8Few<128>::kWarps, many = head_dim == 64 ? Ak8Shape<64>::kWarps : Ak8Shape<128>::kWarps;
+    const size_t rows = std::max<int64_t>(few * std::min<int64_t>(4, rows_in_unit), many * std::min<int64_t>(16, rows_in_unit));
+    return plan_bytes() + size_t(2) * kNumSMs * rows * row;
 }
 
 }  // namespace
@@ -315,11 +324,12 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     if (!distinct(seqs->rows, g.q_heads, cache->head_dim, g.out_row_stride, g.out_head_stride))
         return op_errorf("%s: the strides of out make its heads overlap", who);
     if (g.q == g.out) return op_errorf("%s: out must not be q", who);
-    const int group = g.q_heads / cache->kv_heads, tile_rows = unit_rows(g.type);
+    const int group = g.q_heads / cache->kv_heads;
+    const AttnForm f = attn_form(cache->head_dim, cache->format, g.type, seqs->rows, seqs->n_seqs, group);
     const int64_t jobs = int64_t(seqs->rows) * g.q_heads;
     if (jobs > (int64_t(1) << 33)) return op_errorf("%s: rows * q_heads is above 2^33", who);
     // the plan counts tiles in 32 bits
-    const int64_t blocks = int64_t(seqs->rows) * group / tile_rows + seqs->n_seqs;
+    const int64_t blocks = int64_t(seqs->rows) * group / f.tile_rows + seqs->n_seqs;
     if (blocks * (cache->pages_per_slot / 2 + 1) > INT64_C(0x7fffffff))
         return op_errorf("%s: rows times positions of the page table are above 2^31 tiles: split the call", who);
     int dev = -1, *status = nullptr;
@@ -329,25 +339,29 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     p.seqs = *seqs;
     p.a = g;
     p.group = group;
-    p.workers = kNumSMs * warps_of(cache->head_dim);
-    p.tile_rows = tile_rows;
-    p.part_rows = int(std::min<int64_t>(tile_rows, int64_t(seqs->rows) * group));
+    p.runs = kNumSMs * f.warps / cache->kv_heads;
+    p.tile_rows = f.tile_rows;
+    p.part_rows = int(std::min<int64_t>(f.tile_rows, int64_t(seqs->rows) * group));
+    // A CTA a unit where they fit the machine at once and no warp gets long: one launch.  (Tiles are 32 positions.)
+    const int64_t units = (int64_t(seqs->rows) * group / f.tile_rows + seqs->n_seqs) * cache->kv_heads;
+    const bool direct = units <= kNumSMs && cache->pages_per_slot <= 2 * 8 * f.warps;
     p.vec_q = vec_ok(g.q, g.q_row_stride, g.q_head_stride, g.type);
     p.vec_out = vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
     p.plan = static_cast<uint32_t *>(g.workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(g.workspace) + plan_bytes());
     p.status = status;
-    const AttnKernel kernel = attn_kernel(cache->head_dim, cache->format, g.type != MOSSGPU_BF16);
-    const int smem = attn_smem(cache->head_dim, seqs->n_seqs);
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, attn_smem(cache->head_dim, kAk8MaxSeqs));
+    const auto kernel = direct ? f.direct : f.kernel;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         f.ring + int(sizeof(uint32_t)) * (kAk8MaxSeqs + 1));
     if (e != cudaSuccess) return op_errorf("%s: cudaFuncSetAttribute: %s", who, cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(kNumSMs);
-    cfg.blockDim = dim3(unsigned(warps_of(cache->head_dim)) * 32);
-    cfg.dynamicSmemBytes = size_t(smem);
+    cfg.gridDim = dim3(direct ? unsigned(units) : unsigned(kNumSMs));
+    cfg.blockDim = dim3(unsigned(f.warps) * 32);
+    cfg.dynamicSmemBytes = size_t(f.ring) + sizeof(uint32_t) * (seqs->n_seqs + 1);
     cfg.stream = static_cast<cudaStream_t>(cuda_stream);
     e = cudaLaunchKernelEx(&cfg, kernel, p);
     if (e != cudaSuccess) return op_errorf("%s launch: %s", who, cudaGetErrorString(e));
+    if (direct) return 0;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;

@@ -25,6 +25,7 @@
 #include <type_traits>
 
 #include "../../include/mossgpu.h"
+#include "f32x2.cuh"
 #include "op_support.h"
 
 namespace mossgpu {
@@ -60,36 +61,6 @@ __device__ __forceinline__ float order_value(uint32_t k) {
 }
 __device__ __forceinline__ unsigned long long order_key(float x, int id) {
     return (unsigned long long)order_bits(x) << 32 | uint32_t(~id);
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Two fp32 operations an instruction.
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n add.rn.f32x2 r, a, b;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 r;
-    asm("{\n .reg .b64 a, b, r;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 r, a, b;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 r;
-    asm("{\n .reg .b64 a, b, c, r;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
-        " fma.rn.f32x2 r, a, b, c;\n mov.b64 {%0, %1}, r;\n}"
-        : "=f"(r.x), "=f"(r.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return r;
 }
 
 // Elements 2 i, 2 i + 1 of a vector, and a vector's largest (NaN if it holds one).
