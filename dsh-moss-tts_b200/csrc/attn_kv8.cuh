@@ -165,6 +165,18 @@ __device__ __forceinline__ void load_q8(const void *q, int type, bool vec, int64
     else
         load8(static_cast<const __nv_bfloat16 *>(q) + at, vec, x);
 }
+__device__ __forceinline__ float2 load_q2(const void *q, int type, int64_t at) {
+    if (type == MOSSGPU_F32) {
+        const float *x = static_cast<const float *>(q) + at;
+        return make_float2(x[0], x[1]);
+    }
+    if (type == MOSSGPU_F16) {
+        const __half *x = static_cast<const __half *>(q) + at;
+        return make_float2(__half2float(x[0]), __half2float(x[1]));
+    }
+    const __nv_bfloat16 *x = static_cast<const __nv_bfloat16 *>(q) + at;
+    return make_float2(__bfloat162float(x[0]), __bfloat162float(x[1]));
+}
 __device__ __forceinline__ void store_out8(void *o, int type, bool vec, int64_t at, const float (&x)[8]) {
     if (type == MOSSGPU_F32)
         store8(static_cast<float *>(o) + at, vec, x);
@@ -358,13 +370,312 @@ __device__ __forceinline__ void join_warps(const AttnKv8 &p, const Unit &u, int 
     }
 }
 
-template <int D, int FORMAT, bool SPLIT, bool DIRECT>
+// How a warp's rows enter the products.
+constexpr int kSplit = 0;   // fp16, 8 rows as upper and lower parts: fp32 and fp16 outputs
+constexpr int kHalf = 1;    // fp16, 16 rows: bf16 outputs
+
+// A warp's rows: lane (g, t) has row g of its 8 (kSplit), or rows g and g + 8.
+template <int D, int MODE>
+struct Rows {
+    static constexpr int NR = MODE == kSplit ? 1 : 2;  // rows of a lane
+    static constexpr int NJ = D / 8;                   // output columns of a lane, per row: 2 NJ
+    static constexpr int kRows = 8 * NR;
+    uint32_t q[D / 16][4];
+    float rf[NR];            // what makes a product a score in log2, above 0
+    int new_row[NR];         // which new row of the sequence; -1: none
+    float o[NJ][2 * NR], ref[NR], m[NR], l[NR];
+    int E;                   // biased exponent of the largest V scale so far (scales below 2^-87 lose bits of their weights)
+};
+
+// The query rows from `first` on as fragments; the sign of the scale goes into them.
+template <int D, int MODE>
+__device__ __forceinline__ void load_rows(const AttnKv8 &p, const Unit &u, int first, Rows<D, MODE> &w) {
+    const int lane = threadIdx.x & 31, row8 = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < w.NR; ++r) {
+        const int x = first + row8 + r * 8;
+        float q[D / 64][2][8];
+        float top = 0.f;
+        w.new_row[r] = x < u.n_rows ? x / p.group : -1;
+        const int64_t at = int64_t(u.rr.r0 + x / p.group) * p.a.q_row_stride +
+                           int64_t(u.head * p.group + x % p.group) * p.a.q_head_stride + t * 16;
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                if (w.new_row[r] >= 0) {
+                    load_q8(p.a.q, p.a.type, p.vec_q != 0, at + c * 64 + hf * 8, q[c][hf]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) q[c][hf][i] = 0.f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[c][hf][i]));
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
+        const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
+        w.rf[r] = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float *x4 = &q[c][j / 2][(j & 1) * 4];
+                float2 a = make_float2(x4[0] * to, x4[1] * to), b = make_float2(x4[2] * to, x4[3] * to);
+                if constexpr (MODE == kSplit) {
+                    w.q[c * 4 + j][0] = split2(a, &w.q[c * 4 + j][1]);
+                    w.q[c * 4 + j][2] = split2(b, &w.q[c * 4 + j][3]);
+                } else {
+                    w.q[c * 4 + j][r] = pack2(a);
+                    w.q[c * 4 + j][2 + r] = pack2(b);
+                }
+            }
+        w.m[r] = w.ref[r] = -INFINITY, w.l[r] = 0.f;
+    }
+    w.E = 40;
+#pragma unroll
+    for (int j = 0; j < w.NJ; ++j)
+#pragma unroll
+        for (int i = 0; i < 2 * w.NR; ++i) w.o[j][i] = 0.f;
+}
+
+// One tile for a warp's rows.  st: the stage; ok: bit i says that page i of the tile exists.  Ends with a
+// converged warp that reads the stage no more.
+template <int D, int FORMAT, int MODE>
+__device__ __forceinline__ void tile_rows(const AttnKv8 &p, const Unit &u, uint8_t *st, int tile, uint32_t ok, Rows<D, MODE> &w) {
+    constexpr int NR = Rows<D, MODE>::NR, NJ = Rows<D, MODE>::NJ, kBlock = 16 * D, kChunks = D / 64;
+    const int lane = threadIdx.x & 31, row8 = lane >> 2, t = lane & 3;
+    const float *sc = reinterpret_cast<const float *>(st + 4 * kBlock);  // [k, v][page][16]
+    const int p0 = tile * kAk8Tile;
+    // only tiles that reach into the new rows, or miss a page, have masks
+    const bool whole = p0 + kAk8Tile <= u.span.ctx && ok == 3u;
+    if (!whole) {  // V codes that no position fills become zeros: a weight of 0 has to stay 0
+        if (p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)) {
+#pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                *reinterpret_cast<uint4 *>(st + 2 * kBlock + lane * D + i * 16) = make_uint4(0u, 0u, 0u, 0u);
+        }
+        __syncwarp();
+    }
+
+    // scores, without the rows' factors; pair i = (page, tau) holds two neighbouring positions
+    float2 sv[4][NR];
+    {
+        float c[4][4];  // four chains of products in turn: one alone waits for itself
+#pragma unroll
+        for (int ch = 0; ch < kChunks; ++ch) {
+            uint4 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * (row8 >> 1) + 2 * (i & 1) + (row8 & 1);
+                v[i] = *reinterpret_cast<const uint4 *>(st + (i >> 1) * kBlock + r * D + ch * 64 + t * 16);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t(&qa)[4] = w.q[ch * 4 + j];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t b0, b1;
+                    codes_f16<FORMAT>(j == 0 ? v[i].x : j == 1 ? v[i].y : j == 2 ? v[i].z : v[i].w, b0, b1);
+                    if (ch == 0 && j == 0)
+                        mma16816_0(c[i], qa[0], qa[1], qa[2], qa[3], b0, b1);
+                    else
+                        mma16816(c[i], qa[0], qa[1], qa[2], qa[3], b0, b1);
+                }
+            }
+        }
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+            const float4 ks = *reinterpret_cast<const float4 *>(sc + pg * 16 + 4 * t);
+#pragma unroll
+            for (int tau = 0; tau < 2; ++tau) {
+                const float2 k2 = tau ? make_float2(ks.z, ks.w) : make_float2(ks.x, ks.y);
+                const float(&ci)[4] = c[pg * 2 + tau];
+                if constexpr (MODE == kSplit) {
+                    sv[pg * 2 + tau][0] = mul2(add2(make_float2(ci[0], ci[1]), make_float2(ci[2], ci[3])), k2);
+                } else {
+                    sv[pg * 2 + tau][0] = mul2(make_float2(ci[0], ci[1]), k2);
+                    sv[pg * 2 + tau][1] = mul2(make_float2(ci[2], ci[3]), k2);
+                }
+            }
+        }
+    }
+    uint32_t seen[NR];  // bit: page * 4 + position within the lane's four
+    if (!whole) {
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            seen[r] = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int pos = p0 + (i >> 2) * kKv8Page + 4 * t + (i & 3), j = pos - u.span.ctx;
+                bool in = pos < u.span.total && (ok >> (i >> 2) & 1u);
+                if (in && j >= 0) {
+                    if (w.new_row[r] < 0)
+                        in = false;
+                    else if (!p.a.mask)
+                        in = j <= w.new_row[r];
+                    else
+                        in = j < 32 * p.a.mask_words &&
+                             ((__ldg(p.a.mask + size_t(u.rr.r0 + w.new_row[r]) * p.a.mask_words + j / 32) >> (j & 31)) & 1u);
+                }
+                seen[r] |= in ? 1u << i : 0u;
+                if (!in) ((i & 1) ? sv[i >> 1][r].y : sv[i >> 1][r].x) = -INFINITY;
+            }
+        }
+    }
+    // the running exponent of the V scales
+    {
+        uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
+        if (b >= 0x7f800000u || p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
+        w.E = max(w.E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+    }
+    float corr[NR];
+    // softmax
+#pragma unroll
+    for (int r = 0; r < NR; ++r) {
+        float mx = fmaxf(fmaxf(fmaxf(sv[0][r].x, sv[0][r].y), fmaxf(sv[1][r].x, sv[1][r].y)),
+                         fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        w.m[r] = fmaxf(w.m[r], mx * w.rf[r]);
+        const float now = w.m[r] == -INFINITY ? -INFINITY : w.m[r] - float(140 - w.E);
+        const float use = now == -INFINITY ? 0.f : now;  // what the weights are relative to
+        corr[r] = ex2(w.ref[r] - use);
+        w.ref[r] = now;
+        const float2 rf2 = make_float2(w.rf[r], w.rf[r]), off = make_float2(-use, -use);
+        float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float2 &x = sv[i][r];
+            x = fma2(x, rf2, off);
+            x.x = ex2(x.x), x.y = ex2(x.y);
+            sum = add2(sum, x);
+        }
+        w.l[r] = fmaf(w.l[r], corr[r], sum.x + sum.y);
+    }
+    // weights as the left operand
+    uint32_t wa[2][4];  // [page]: tau 0 rows g, g + 8, tau 1 rows g, g + 8
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) {
+        const float4 vs = *reinterpret_cast<const float4 *>(sc + 32 + pg * 16 + 4 * t);
+#pragma unroll
+        for (int tau = 0; tau < 2; ++tau) {
+            const float2 v2 = tau ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y);
+            float2 x[NR];
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                x[r] = mul2(sv[pg * 2 + tau][r], v2);
+                if (!whole) {  // a masked position's scale may be anything, NaN included
+                    if (!(seen[r] >> (pg * 4 + tau * 2) & 1u)) x[r].x = 0.f;
+                    if (!(seen[r] >> (pg * 4 + tau * 2 + 1) & 1u)) x[r].y = 0.f;
+                }
+            }
+            if constexpr (MODE == kSplit) {
+                wa[pg][tau * 2] = split2(x[0], &wa[pg][tau * 2 + 1]);
+            } else {
+                wa[pg][tau * 2] = pack2(x[0]);
+                wa[pg][tau * 2 + 1] = pack2(x[1]);
+            }
+        }
+    }
+    if constexpr (MODE != kSplit) {
+        // most tiles raise no maximum
+        if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[NR - 1] != 1.f)) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+                w.o[j][0] *= corr[0], w.o[j][1] *= corr[0];
+                w.o[j][2 * NR - 2] *= corr[NR - 1], w.o[j][2 * NR - 1] *= corr[NR - 1];
+            }
+        }
+    }
+    uint32_t vw[2][4][D / 32];  // [page][position][word]
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint8_t *from = st + (2 + pg) * kBlock + (4 * t + i) * D + row8 * (D / 8);
+            if constexpr (D == 64) {
+                const uint2 v = *reinterpret_cast<const uint2 *>(from);
+                vw[pg][i][0] = v.x, vw[pg][i][1] = v.y;
+            } else {
+                const uint4 v = *reinterpret_cast<const uint4 *>(from);
+                vw[pg][i][0] = v.x, vw[pg][i][1] = v.y, vw[pg][i][2] = v.z, vw[pg][i][3] = v.w;
+            }
+        }
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            uint32_t b0[2][2], b1[2][2];  // [page], of columns 4 k + 2 half and the next
+#pragma unroll
+            for (int pg = 0; pg < 2; ++pg) {
+                codes_f16<FORMAT>(__byte_perm(vw[pg][0][k], vw[pg][1][k], half ? 0x7362 : 0x5140), b0[pg][0], b0[pg][1]);
+                codes_f16<FORMAT>(__byte_perm(vw[pg][2][k], vw[pg][3][k], half ? 0x7362 : 0x5140), b1[pg][0], b1[pg][1]);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float(&oj)[2 * NR] = w.o[4 * k + 2 * half + i];
+                if constexpr (MODE == kSplit) {
+                    float c[4];
+                    mma16816_0(c, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b0[0][i], b1[0][i]);
+                    mma16816(c, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b0[1][i], b1[1][i]);
+                    const float2 y = fma2(make_float2(oj[0], oj[1]), make_float2(corr[0], corr[0]),
+                                          add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
+                    oj[0] = y.x, oj[1] = y.y;
+                } else {
+                    mma16816(oj, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b0[0][i], b1[0][i]);
+                    mma16816(oj, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b0[1][i], b1[1][i]);
+                }
+            }
+        }
+    }
+    __syncwarp();
+}
+
+// A warp's rows (from `first` on) to the output where `part` is NULL, else as sums, R and l to part[row].
+// Lane (g, t) has of its rows the elements 2 NJ t .. in two runs of NJ.
+template <int D, int MODE>
+__device__ __forceinline__ void finish_rows(const AttnKv8 &p, const Unit &u, int first, float *part, Rows<D, MODE> &w) {
+    constexpr int NJ = Rows<D, MODE>::NJ;
+    const int lane = threadIdx.x & 31, row8 = lane >> 2, t = lane & 3;
+#pragma unroll
+    for (int r = 0; r < w.NR; ++r) {
+        w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 1);
+        w.l[r] += __shfl_xor_sync(0xffffffffu, w.l[r], 2);
+        if (w.new_row[r] < 0) continue;
+        const int x = first + row8 + r * 8;
+        if (!part) {
+            const float f = w.l[r] == 0.f ? 0.f : 1.f / w.l[r];
+            const int64_t at = int64_t(u.rr.r0 + w.new_row[r]) * p.a.out_row_stride +
+                               int64_t(u.head * p.group + x % p.group) * p.a.out_head_stride + t * (2 * NJ);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < NJ; j += 8) {
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) y[i] = w.o[j + i][2 * r + e] * f;
+                    store_out8(p.a.out, p.a.type, p.vec_out != 0, at + e * NJ + j, y);
+                }
+        } else {
+            float *to = part + (row8 + r * 8) * (D + 4);
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < NJ; j += 4)
+                    *reinterpret_cast<float4 *>(to + t * (2 * NJ) + e * NJ + j) =
+                        make_float4(w.o[j][2 * r + e], w.o[j + 1][2 * r + e], w.o[j + 2][2 * r + e], w.o[j + 3][2 * r + e]);
+            if (t == 0) to[D] = w.ref[r], to[D + 1] = w.l[r];
+        }
+    }
+}
+
+// Units of the rows that one warp takes.
+template <int D, int FORMAT, int MODE, bool DIRECT>
 __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const __grid_constant__ AttnKv8 p) {
     using S = Ak8Shape<D>;
-    constexpr int kRows = SPLIT ? 8 : 16;      // rows of a unit
-    constexpr int NR = SPLIT ? 1 : 2;          // rows a lane holds
-    constexpr int NJ = D / 8;                  // output columns a lane holds, per row: 2 NJ
-    constexpr int kChunks = D / 64;            // 64-wide chunks of a row
+    using W = Rows<D, MODE>;
     extern __shared__ __align__(16) uint8_t smem[];
     uint32_t *plan = reinterpret_cast<uint32_t *>(smem + S::kRing);  // [n_seqs + 1]
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -373,29 +684,24 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
     Run run{};
     run.g_end = 1;
     if (!DIRECT) {
-        const int64_t total = plan_tiles<kRows, kAk8Tile, S::kWarps>(p, plan);
+        const int64_t total = plan_tiles<W::kRows, kAk8Tile, S::kWarps>(p, plan);
         if (!warp_run<S::kWarps>(p, total, run)) return;
     }
-
     uint8_t *ring = smem + warp * (S::kStage * S::kStages);
-    const int row8 = lane >> 2, t = lane & 3;  // the lane's row and column group in a product
     const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(ring));
 
     while (run.g < run.g_end) {
         int status = 0;
-        const Unit u = DIRECT ? direct_unit<kRows>(p, blockIdx.x, kAk8Tile, &status) : find_unit(p, plan, run, kAk8Tile);
+        const Unit u = DIRECT ? direct_unit<W::kRows>(p, blockIdx.x, kAk8Tile, &status) : find_unit(p, plan, run, kAk8Tile);
         if (DIRECT && u.n_rows == 0) return;  // the whole CTA
-        const RowRange rr = u.rr;
-        const SeqSpan span = u.span;
-        const int head = u.head, block = u.block, t1 = u.t1, n_rows = u.n_rows;
-        const int t0 = u.t0 + (DIRECT ? warp : 0), step = DIRECT ? S::kWarps : 1;  // this warp's tiles
+        const int t1 = u.t1, t0 = u.t0 + (DIRECT ? warp : 0), step = DIRECT ? S::kWarps : 1;  // this warp's tiles
 
         // ---- the copies of a tile: lane i has the id of page i & 1, loaded a tile ahead of its use
         const auto page_id = [&](int tile) {
             const int i = 2 * tile + (lane & 1);
             return tile < t1 && i < u.n_pages ? kv8_page(p.cache, __ldg(u.table + i), &status) : -1;
         };
-        const auto issue = [&](int stage, int id) { copy_pages<D, 2>(p.cache, head, ring_s + stage * S::kStage, id); };
+        const auto issue = [&](int stage, int id) { copy_pages<D, 2>(p.cache, u.head, ring_s + stage * S::kStage, id); };
         int ids[S::kStages];
 #pragma unroll
         for (int i = 0; i < S::kStages; ++i) ids[i] = page_id(t0 + i * step);
@@ -404,64 +710,11 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
             if (t0 + i * step < t1) issue(i, ids[i]);
             cp_async_commit();
         }
-
-        // ---- the query rows as fragments; the sign of the scale goes into them
-        uint32_t qf[D / 16][4];
-        float rf[NR];           // what makes a product a score in log2, above 0
-        int new_row[NR];        // which new row of the sequence; -1: none
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            const int x = block * kRows + row8 + r * 8;
-            float q[kChunks][2][8];
-            float top = 0.f;
-            new_row[r] = x < n_rows ? x / p.group : -1;
-            const int64_t at = int64_t(rr.r0 + x / p.group) * p.a.q_row_stride +
-                               int64_t(head * p.group + x % p.group) * p.a.q_head_stride + t * 16;
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    if (new_row[r] >= 0) {
-                        load_q8(p.a.q, p.a.type, p.vec_q != 0, at + c * 64 + hf * 8, q[c][hf]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) q[c][hf][i] = 0.f;
-                    }
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(q[c][hf][i]));
-                }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
-            const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
-            rf[r] = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
-#pragma unroll
-            for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float *x4 = &q[c][j / 2][(j & 1) * 4];
-                    if constexpr (SPLIT) {
-                        qf[c * 4 + j][0] = split2(make_float2(x4[0] * to, x4[1] * to), &qf[c * 4 + j][1]);
-                        qf[c * 4 + j][2] = split2(make_float2(x4[2] * to, x4[3] * to), &qf[c * 4 + j][3]);
-                    } else {
-                        qf[c * 4 + j][r] = pack2(make_float2(x4[0] * to, x4[1] * to));
-                        qf[c * 4 + j][2 + r] = pack2(make_float2(x4[2] * to, x4[3] * to));
-                    }
-                }
-        }
-
-        float o[NJ][2 * NR], ref[NR], m[NR], l[NR];
-        int E = 40;  // biased exponent of the largest V scale so far (scales below 2^-87 lose bits of their weights)
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < 2 * NR; ++i) o[j][i] = 0.f;
-#pragma unroll
-        for (int r = 0; r < NR; ++r) m[r] = ref[r] = -INFINITY, l[r] = 0.f;
-
+        W w;
+        load_rows<D, MODE>(p, u, u.block * W::kRows, w);
         int stage = 0;
         for (int tile = t0; tile < t1; tile += step) {
-            const int id_now = ids[0];
+            const uint32_t ok = __ballot_sync(0xffffffffu, ids[0] >= 0) & 3u;
             {
                 int st = stage + S::kStages - 1;
                 if (st >= S::kStages) st -= S::kStages;
@@ -473,227 +726,339 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
             }
             cp_async_wait<S::kStages - 1>();
             __syncwarp();
-            uint8_t *st = ring + stage * S::kStage;
-            const float *sc = reinterpret_cast<const float *>(st + 4 * S::kBlock);  // [k, v][page][16]
-            const int p0 = tile * kAk8Tile;
-            const uint32_t ok = __ballot_sync(0xffffffffu, id_now >= 0) & 3u;
-            // only tiles that reach into the new rows, or miss a page, have masks
-            const bool whole = p0 + kAk8Tile <= span.ctx && ok == 3u;
-            if (!whole) {  // V codes that no position fills become zeros: a weight of 0 has to stay 0
-                if (p0 + lane >= span.total || !(ok >> (lane >> 4) & 1u)) {
-#pragma unroll
-                    for (int i = 0; i < D / 16; ++i)
-                        *reinterpret_cast<uint4 *>(st + 2 * S::kBlock + lane * D + i * 16) = make_uint4(0u, 0u, 0u, 0u);
-                }
-                __syncwarp();
-            }
+            tile_rows<D, FORMAT, MODE>(p, u, ring + stage * S::kStage, tile, ok, w);
+            if (++stage == S::kStages) stage = 0;
+        }
+        op_report(p.status, status);
+        if (DIRECT) {
+            finish_rows<D, MODE>(p, u, u.block * W::kRows, reinterpret_cast<float *>(ring), w);
+            __syncthreads();
+            join_warps<D, S::kWarps>(p, u, W::kRows, reinterpret_cast<const float *>(smem), S::kStage * S::kStages / 4);
+            return;
+        }
+        finish_rows<D, MODE>(p, u, u.block * W::kRows,
+                             u.t0 == 0 && t1 == u.tiles ? nullptr
+                                                        : p.part + size_t(2 * run.item + (u.t0 == 0 ? 1 : 0)) * p.part_rows * (D + 4),
+                             w);
+        run.g += t1 - t0;
+    }
+}
 
-            // scores, without the rows' factors; pair i = (page, tau) holds two neighbouring positions
-            float2 sv[4][NR];
+// Units of more rows.  A CTA's four warps take 8 or 16 of them each; a tile is read once for all of
+// them, and its codes are converted to fp16 once, each thread its share, a tile ahead of its use (the
+// conversions are as many instructions as the rest of a tile's work).  The warps take their fragments
+// from the converted tile with ldmatrix; its 16-byte chunks are stored at chunk ^ (row % 8).  A run
+// belongs to a CTA.
+template <int D>
+struct Ak8Block {
+    static constexpr int kWarps = 4, kCtas = 3, kStages = 4;  // CTAs of an SM
+    static constexpr int kStage = 64 * D + 256;               // a tile as it is in the cache: 32 rows of K, of V, scales
+    static constexpr int kTile = 128 * D;                     // the same in fp16
+    static constexpr int kRing = kStage * kStages + 2 * kTile;
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t at) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
+}
+
+// A thread's share of a tile's codes, to fp16.  Positions that do not exist become zeros.
+template <int D, int FORMAT>
+__device__ __forceinline__ void convert_tile(const uint8_t *raw, uint8_t *to, int left, uint32_t ok) {
+    constexpr int kGran = D / 16;  // 16-byte granules of a row of codes
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg) {
-                const float4 ks = *reinterpret_cast<const float4 *>(sc + pg * 16 + 4 * t);
+    for (int i = 0; i < 64 * kGran / 128; ++i) {
+        const int at = int(threadIdx.x) + i * 128, row = at / kGran, gr = at % kGran, pos = row & 31;
+        uint4 w = *reinterpret_cast<const uint4 *>(raw + at * 16);
+        if (pos >= left || !(ok >> (pos >> 4) & 1u)) w = make_uint4(0u, 0u, 0u, 0u);
+        uint4 a, b;
+        codes_f16<FORMAT>(w.x, a.x, a.y);
+        codes_f16<FORMAT>(w.y, a.z, a.w);
+        codes_f16<FORMAT>(w.z, b.x, b.y);
+        codes_f16<FORMAT>(w.w, b.z, b.w);
+        *reinterpret_cast<uint4 *>(to + row * (2 * D) + ((2 * gr) ^ (row & 7)) * 16) = a;
+        *reinterpret_cast<uint4 *>(to + row * (2 * D) + ((2 * gr + 1) ^ (row & 7)) * 16) = b;
+    }
+}
+
+template <int D, int FORMAT, int MODE>
+__global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(const __grid_constant__ AttnKv8 p) {
+    using S = Ak8Block<D>;
+    constexpr int NR = MODE == kSplit ? 1 : 2, kWarpRows = 8 * NR, kRows = S::kWarps * kWarpRows, kBlock = 16 * D;
+    extern __shared__ __align__(16) uint8_t smem[];
+    uint32_t *plan = reinterpret_cast<uint32_t *>(smem + S::kRing);
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, row8 = lane >> 2, t = lane & 3, H = p.cache.kv_heads;
+    const int64_t total = plan_tiles<kRows, kAk8Tile, S::kWarps>(p, plan);
+    const int used = runs_used(total, p.runs);
+    const uint32_t ring_s = static_cast<uint32_t>(__cvta_generic_to_shared(smem)), half_s = ring_s + S::kStage * S::kStages;
+    const uint32_t page_bytes = uint32_t(2 * kBlock) * uint32_t(H);
+
+    for (int item = blockIdx.x; item < used * H; item += gridDim.x) {
+        Run run;
+        run.item = item;
+        run.head = item % H;
+        run.g = run_begin(total, used, item / H);
+        run.g_end = run_begin(total, used, item / H + 1);
+        while (run.g < run.g_end) {
+            int status = 0;
+            const Unit u = find_unit(p, plan, run, kAk8Tile);
+            const int t0 = u.t0, t1 = u.t1;
+            const auto page_id = [&](int tile) {
+                const int i = 2 * tile + (lane & 1);
+                return tile < t1 && i < u.n_pages ? kv8_page(p.cache, __ldg(u.table + i), &status) : -1;
+            };
+            // warp i copies page i & 1's K (i < 2) or V, and its scales
+            const auto issue = [&](int tile, int id) {
+                const int page = __shfl_sync(0xffffffffu, id, warp & 1);
+                if (page >= 0) {
+                    const uint32_t dst = ring_s + ((tile - t0) % S::kStages) * S::kStage;
+                    const uint8_t *from = static_cast<const uint8_t *>(p.cache.codes) + uint64_t(uint32_t(page)) * page_bytes +
+                                          uint32_t((warp >= 2 ? page_bytes / 2 : 0u) + u.head * kBlock + lane * 16);
 #pragma unroll
-                for (int tau = 0; tau < 2; ++tau) {
-                    const int r = 4 * (row8 >> 1) + 2 * tau + (row8 & 1);
-                    float c[4];
-#pragma unroll
-                    for (int ch = 0; ch < kChunks; ++ch) {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(st + pg * S::kBlock + r * D + ch * 64 + t * 16);
-                        const uint32_t ww[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            uint32_t b0, b1;
-                            codes_f16<FORMAT>(ww[j], b0, b1);
-                            const uint32_t(&qa)[4] = qf[ch * 4 + j];
-                            if (ch == 0 && j == 0)
-                                mma16816_0(c, qa[0], qa[1], qa[2], qa[3], b0, b1);
-                            else
-                                mma16816(c, qa[0], qa[1], qa[2], qa[3], b0, b1);
-                        }
-                    }
-                    const float2 k2 = tau ? make_float2(ks.z, ks.w) : make_float2(ks.x, ks.y);
-                    if constexpr (SPLIT) {
-                        sv[pg * 2 + tau][0] = mul2(add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])), k2);
-                    } else {
-                        sv[pg * 2 + tau][0] = mul2(make_float2(c[0], c[1]), k2);
-                        sv[pg * 2 + tau][1] = mul2(make_float2(c[2], c[3]), k2);
+                    for (int i = 0; i < kBlock / 512; ++i) cp_async16(dst + warp * kBlock + lane * 16 + i * 512, from + i * 512);
+                    if (lane < 4) {
+                        const float *s = p.cache.scales + uint64_t(uint32_t(page)) * uint32_t(2 * kKv8Page * H) +
+                                         uint32_t(((warp >= 2 ? H : 0) + u.head) * kKv8Page + lane * 4);
+                        cp_async16(dst + 4 * kBlock + warp * 64 + lane * 16, s);
                     }
                 }
-            }
-            uint32_t seen[NR];  // bit: page * 4 + position within the lane's four
-            if (!whole) {
+                cp_async_commit();
+            };
+            const auto pages_ok = [&](int id) { return __ballot_sync(0xffffffffu, id >= 0) & 3u; };
+            int ids[S::kStages];  // of tiles t, t + 1, ..
 #pragma unroll
-                for (int r = 0; r < NR; ++r) {
-                    seen[r] = 0;
+            for (int i = 0; i < S::kStages; ++i) ids[i] = page_id(t0 + i);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int pos = p0 + (i >> 2) * kKv8Page + 4 * t + (i & 3), j = pos - span.ctx;
-                        bool in = pos < span.total && (ok >> (i >> 2) & 1u);
-                        if (in && j >= 0) {
-                            if (new_row[r] < 0)
-                                in = false;
-                            else if (!p.a.mask)
-                                in = j <= new_row[r];
-                            else
-                                in = j < 32 * p.a.mask_words &&
-                                     ((__ldg(p.a.mask + size_t(rr.r0 + new_row[r]) * p.a.mask_words + j / 32) >> (j & 31)) & 1u);
-                        }
-                        seen[r] |= in ? 1u << i : 0u;
-                        if (!in) ((i & 1) ? sv[i >> 1][r].y : sv[i >> 1][r].x) = -INFINITY;
-                    }
-                }
-            }
-            // the running exponent of the V scales
-            {
-                uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
-                if (b >= 0x7f800000u || p0 + lane >= span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
-                E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
-            }
-            // softmax
-            float corr[NR];
+            for (int i = 0; i < S::kStages - 1; ++i) issue(t0 + i, ids[i]);
+
+            // ---- the query rows as fragments; the sign of the scale goes into them
+            const int first = u.block * kRows + warp * kWarpRows;
+            const bool any = first < u.n_rows;  // else the warp only copies and converts
+            uint32_t q[D / 16][4];
+            float rf[NR], ref[NR], m[NR], l[NR], o[D / 8][2 * NR];
+            int new_row[NR], E = 40;
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
-                float mx = fmaxf(fmaxf(fmaxf(sv[0][r].x, sv[0][r].y), fmaxf(sv[1][r].x, sv[1][r].y)),
-                                 fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                m[r] = fmaxf(m[r], mx * rf[r]);
-                const float now = m[r] == -INFINITY ? -INFINITY : m[r] - float(140 - E);
-                const float use = now == -INFINITY ? 0.f : now;
-                corr[r] = ex2(ref[r] - use);
-                ref[r] = now;
-                const float2 rf2 = make_float2(rf[r], rf[r]), off = make_float2(-use, -use);
-                float2 sum = make_float2(0.f, 0.f);
+                const int x = first + row8 + r * 8;
+                new_row[r] = x < u.n_rows ? x / p.group : -1;
+                const int64_t at = int64_t(u.rr.r0 + x / p.group) * p.a.q_row_stride +
+                                   int64_t(u.head * p.group + x % p.group) * p.a.q_head_stride + 2 * t;
+                float2 v[D / 8];
+                float top = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float2 &x = sv[i][r];
-                    x = fma2(x, rf2, off);
-                    x.x = ex2(x.x), x.y = ex2(x.y);
-                    sum = add2(sum, x);
+                for (int i = 0; i < D / 8; ++i) {
+                    v[i] = new_row[r] >= 0 ? load_q2(p.a.q, p.a.type, at + i * 8) : make_float2(0.f, 0.f);
+                    top = fmaxf(top, fmaxf(fabsf(v[i].x), fabsf(v[i].y)));
                 }
-                l[r] = fmaf(l[r], corr[r], sum.x + sum.y);
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
+                const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
+                rf[r] = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) {
+                    const float2 y = make_float2(v[i].x * to, v[i].y * to);
+                    if constexpr (MODE == kSplit)
+                        q[i / 2][2 * (i & 1)] = split2(y, &q[i / 2][2 * (i & 1) + 1]);
+                    else
+                        q[i / 2][2 * (i & 1) + r] = pack2(y);
+                }
+                m[r] = ref[r] = -INFINITY, l[r] = 0.f;
             }
-            // weights as the left operand: tau 0 rows g, g + 8, tau 1 rows g, g + 8
-            uint32_t wa[2][4];
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg) {
-                const float4 vs = *reinterpret_cast<const float4 *>(sc + 32 + pg * 16 + 4 * t);
+            for (int j = 0; j < D / 8; ++j)
 #pragma unroll
-                for (int tau = 0; tau < 2; ++tau) {
-                    const float2 v2 = tau ? make_float2(vs.z, vs.w) : make_float2(vs.x, vs.y);
-                    float2 w[NR];
+                for (int i = 0; i < 2 * NR; ++i) o[j][i] = 0.f;
+
+            cp_async_wait<S::kStages - 2>();
+            __syncthreads();
+            convert_tile<D, FORMAT>(smem, smem + S::kStage * S::kStages, u.span.total - t0 * kAk8Tile, pages_ok(ids[0]));
+            for (int tile = t0; tile < t1; ++tile) {
+                const uint32_t ok = pages_ok(ids[0]);
+                cp_async_wait<S::kStages - 3>();
+                __syncthreads();  // tile is converted and tile + 1 has arrived for all; tile - 1 is read by none
+                issue(tile + S::kStages - 1, ids[S::kStages - 1]);
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        w[r] = mul2(sv[pg * 2 + tau][r], v2);
-                        if (!whole) {  // a masked position's scale may be anything, NaN included
-                            if (!(seen[r] >> (pg * 4 + tau * 2) & 1u)) w[r].x = 0.f;
-                            if (!(seen[r] >> (pg * 4 + tau * 2 + 1) & 1u)) w[r].y = 0.f;
+                for (int i = 0; i < S::kStages - 1; ++i) ids[i] = ids[i + 1];
+                ids[S::kStages - 1] = page_id(tile + S::kStages);
+                if (tile + 1 < t1)
+                    convert_tile<D, FORMAT>(smem + ((tile + 1 - t0) % S::kStages) * S::kStage,
+                                            smem + S::kStage * S::kStages + ((tile + 1 - t0) & 1) * S::kTile,
+                                            u.span.total - (tile + 1) * kAk8Tile, pages_ok(ids[0]));
+                if (!any) continue;
+                const float *sc = reinterpret_cast<const float *>(smem + ((tile - t0) % S::kStages) * S::kStage + 4 * kBlock);  // [k, v][32]
+                const uint32_t tile_s = half_s + ((tile - t0) & 1) * S::kTile;
+                const int p0 = tile * kAk8Tile;
+                const bool whole = p0 + kAk8Tile <= u.span.ctx && ok == 3u;
+
+                // scores without the rows' factors: of positions 8 j + 2 t and the next
+                float2 sv[4][NR];
+                {
+                    float c[4][4];  // four chains of products in turn: one alone waits for itself
+#pragma unroll
+                    for (int k = 0; k < D / 32; ++k) {
+                        uint32_t b[4][4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            ldmatrix4(b[j], tile_s + (8 * j + (lane & 7)) * (2 * D) + ((4 * k + (lane >> 3)) ^ (lane & 7)) * 16);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            if (k == 0)
+                                mma16816_0(c[j], q[0][0], q[0][1], q[0][2], q[0][3], b[j][0], b[j][1]);
+                            else
+                                mma16816(c[j], q[2 * k][0], q[2 * k][1], q[2 * k][2], q[2 * k][3], b[j][0], b[j][1]);
+                        }
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            mma16816(c[j], q[2 * k + 1][0], q[2 * k + 1][1], q[2 * k + 1][2], q[2 * k + 1][3], b[j][2], b[j][3]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 k2 = *reinterpret_cast<const float2 *>(sc + 8 * j + 2 * t);
+                        if constexpr (MODE == kSplit) {
+                            sv[j][0] = mul2(add2(make_float2(c[j][0], c[j][1]), make_float2(c[j][2], c[j][3])), k2);
+                        } else {
+                            sv[j][0] = mul2(make_float2(c[j][0], c[j][1]), k2);
+                            sv[j][NR - 1] = mul2(make_float2(c[j][2], c[j][3]), k2);
                         }
                     }
-                    if constexpr (SPLIT) {
-                        wa[pg][tau * 2] = split2(w[0], &wa[pg][tau * 2 + 1]);
+                }
+                uint32_t seen[NR];  // bit: 2 j + (0 or 1)
+                if (!whole) {
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        seen[r] = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const int pos = p0 + 8 * (i >> 1) + 2 * t + (i & 1), j = pos - u.span.ctx;
+                            bool in = pos < u.span.total && (ok >> (i >> 2) & 1u);
+                            if (in && j >= 0) {
+                                if (new_row[r] < 0)
+                                    in = false;
+                                else if (!p.a.mask)
+                                    in = j <= new_row[r];
+                                else
+                                    in = j < 32 * p.a.mask_words &&
+                                         ((__ldg(p.a.mask + size_t(u.rr.r0 + new_row[r]) * p.a.mask_words + j / 32) >> (j & 31)) & 1u);
+                            }
+                            seen[r] |= in ? 1u << i : 0u;
+                            if (!in) ((i & 1) ? sv[i >> 1][r].y : sv[i >> 1][r].x) = -INFINITY;
+                        }
+                    }
+                }
+                {
+                    uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
+                    if (b >= 0x7f800000u || p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
+                    E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+                }
+                float corr[NR];
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
+                    float mx = fmaxf(fmaxf(fmaxf(sv[0][r].x, sv[0][r].y), fmaxf(sv[1][r].x, sv[1][r].y)),
+                                     fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+                    m[r] = fmaxf(m[r], mx * rf[r]);
+                    const float now = m[r] == -INFINITY ? -INFINITY : m[r] - float(140 - E);
+                    const float use = now == -INFINITY ? 0.f : now;
+                    corr[r] = ex2(ref[r] - use);
+                    ref[r] = now;
+                    const float2 rf2 = make_float2(rf[r], rf[r]), off = make_float2(-use, -use);
+                    float2 sum = make_float2(0.f, 0.f);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        float2 &x = sv[j][r];
+                        x = fma2(x, rf2, off);
+                        x.x = ex2(x.x), x.y = ex2(x.y);
+                        sum = add2(sum, x);
+                    }
+                    l[r] = fmaf(l[r], corr[r], sum.x + sum.y);
+                }
+                uint32_t wa[2][4];  // the weights as the left operand, 16 positions each
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float2 v2 = *reinterpret_cast<const float2 *>(sc + 32 + 8 * j + 2 * t);
+                    float2 x[NR];
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        x[r] = mul2(sv[j][r], v2);
+                        if (!whole) {  // a masked position's scale may be anything, NaN included
+                            if (!(seen[r] >> (2 * j) & 1u)) x[r].x = 0.f;
+                            if (!(seen[r] >> (2 * j + 1) & 1u)) x[r].y = 0.f;
+                        }
+                    }
+                    if constexpr (MODE == kSplit) {
+                        wa[j / 2][2 * (j & 1)] = split2(x[0], &wa[j / 2][2 * (j & 1) + 1]);
                     } else {
-                        wa[pg][tau * 2] = pack2(w[0]);
-                        wa[pg][tau * 2 + 1] = pack2(w[1]);
+                        wa[j / 2][2 * (j & 1)] = pack2(x[0]);
+                        wa[j / 2][2 * (j & 1) + 1] = pack2(x[NR - 1]);
                     }
                 }
-            }
-            if constexpr (!SPLIT) {
-                // the sums stay in the products' accumulators; most tiles raise no maximum
-                if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[1] != 1.f)) {
+                if constexpr (MODE == kHalf) {
+                    // the sums stay in the products' accumulators; most tiles raise no maximum
+                    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[NR - 1] != 1.f)) {
 #pragma unroll
-                    for (int j = 0; j < NJ; ++j) {
-                        o[j][0] *= corr[0], o[j][1] *= corr[0];
-                        o[j][2] *= corr[1], o[j][3] *= corr[1];
+                        for (int j = 0; j < D / 8; ++j) {
+                            o[j][0] *= corr[0], o[j][1] *= corr[0];
+                            o[j][2 * NR - 2] *= corr[NR - 1], o[j][2 * NR - 1] *= corr[NR - 1];
+                        }
                     }
                 }
-            }
-            uint32_t vw[2][4][D / 32];  // [page][position][word]
+                const uint32_t v_s = tile_s + (32 + (lane & 15)) * (2 * D);  // the lane's row of the first 16
 #pragma unroll
-            for (int pg = 0; pg < 2; ++pg)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint8_t *from = st + (2 + pg) * S::kBlock + (4 * t + i) * D + row8 * (D / 8);
-                    if constexpr (D == 64) {
-                        const uint2 w = *reinterpret_cast<const uint2 *>(from);
-                        vw[pg][i][0] = w.x, vw[pg][i][1] = w.y;
-                    } else {
-                        const uint4 w = *reinterpret_cast<const uint4 *>(from);
-                        vw[pg][i][0] = w.x, vw[pg][i][1] = w.y, vw[pg][i][2] = w.z, vw[pg][i][3] = w.w;
-                    }
-                }
-#pragma unroll
-            for (int w = 0; w < D / 32; ++w)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    uint32_t b0[2][2], b1[2][2];  // [page], of columns 4 w + 2 half and the next
-#pragma unroll
-                    for (int pg = 0; pg < 2; ++pg) {
-                        codes_f16<FORMAT>(__byte_perm(vw[pg][0][w], vw[pg][1][w], half ? 0x7362 : 0x5140), b0[pg][0], b0[pg][1]);
-                        codes_f16<FORMAT>(__byte_perm(vw[pg][2][w], vw[pg][3][w], half ? 0x7362 : 0x5140), b1[pg][0], b1[pg][1]);
-                    }
+                for (int j = 0; j < D / 16; ++j) {  // 16 columns
+                    uint32_t b[2][4];
+                    ldmatrix4_t(b[0], v_s + ((2 * j + (lane >> 4)) ^ (lane & 7)) * 16);
+                    ldmatrix4_t(b[1], v_s + 16 * (2 * D) + ((2 * j + (lane >> 4)) ^ (lane & 7)) * 16);
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        float(&oj)[2 * NR] = o[4 * w + 2 * half + k];
-                        if constexpr (SPLIT) {
+                        float(&oj)[2 * NR] = o[2 * j + k];
+                        if constexpr (MODE == kSplit) {
                             float c[4];
-                            mma16816_0(c, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b0[0][k], b1[0][k]);
-                            mma16816(c, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b0[1][k], b1[1][k]);
+                            mma16816_0(c, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b[0][2 * k], b[0][2 * k + 1]);
+                            mma16816(c, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b[1][2 * k], b[1][2 * k + 1]);
                             const float2 y = fma2(make_float2(oj[0], oj[1]), make_float2(corr[0], corr[0]),
                                                   add2(make_float2(c[0], c[1]), make_float2(c[2], c[3])));
                             oj[0] = y.x, oj[1] = y.y;
                         } else {
-                            mma16816(oj, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b0[0][k], b1[0][k]);
-                            mma16816(oj, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b0[1][k], b1[1][k]);
+                            mma16816(oj, wa[0][0], wa[0][1], wa[0][2], wa[0][3], b[0][2 * k], b[0][2 * k + 1]);
+                            mma16816(oj, wa[1][0], wa[1][1], wa[1][2], wa[1][3], b[1][2 * k], b[1][2 * k + 1]);
                         }
                     }
                 }
-            __syncwarp();  // the stage is free again
-            if (++stage == S::kStages) stage = 0;
-        }
-        op_report(p.status, status);
-
-        // ---- results: lane (g, t) has of its rows the elements 2 NJ t .. in two runs of NJ
-        const bool all = !DIRECT && u.t0 == 0 && t1 == u.tiles;
-        float *part = DIRECT ? reinterpret_cast<float *>(ring) : p.part + size_t(2 * run.item + (u.t0 == 0 ? 1 : 0)) * p.part_rows * (D + 4);
-        if (DIRECT) __syncwarp();  // the ring is read no more
-#pragma unroll
-        for (int r = 0; r < NR; ++r) {
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-            l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-            if (new_row[r] < 0) continue;
-            const int x = block * kRows + row8 + r * 8;
-            if (all) {
-                const float f = l[r] == 0.f ? 0.f : 1.f / l[r];
-                const int64_t at = int64_t(rr.r0 + new_row[r]) * p.a.out_row_stride +
-                                   int64_t(head * p.group + x % p.group) * p.a.out_head_stride + t * (2 * NJ);
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int j = 0; j < NJ; j += 8) {
-                        float y[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) y[i] = o[j + i][2 * r + e] * f;
-                        store_out8(p.a.out, p.a.type, p.vec_out != 0, at + e * NJ + j, y);
-                    }
-            } else {
-                float *to = part + (row8 + r * 8) * (D + 4);
-#pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int j = 0; j < NJ; j += 4)
-                        *reinterpret_cast<float4 *>(to + t * (2 * NJ) + e * NJ + j) =
-                            make_float4(o[j][2 * r + e], o[j + 1][2 * r + e], o[j + 2][2 * r + e], o[j + 3][2 * r + e]);
-                if (t == 0) to[D] = ref[r], to[D + 1] = l[r];
             }
-        }
-        if (DIRECT) {
+            cp_async_wait<0>();
             __syncthreads();
-            join_warps<D, S::kWarps>(p, u, kRows, reinterpret_cast<const float *>(smem), S::kStage * S::kStages / 4);
-            return;
+            op_report(p.status, status);
+
+            // ---- results: lane (g, t) has the elements 8 j + 2 t and the next of its rows
+            const bool all = u.t0 == 0 && t1 == u.tiles;
+            float *part = p.part + (size_t(2 * run.item + (u.t0 == 0 ? 1 : 0)) * p.part_rows + warp * kWarpRows + row8) * (D + 4);
+#pragma unroll
+            for (int r = 0; r < NR; ++r) {
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+                l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+                if (new_row[r] < 0) continue;
+                const int x = first + row8 + r * 8;
+                if (all) {
+                    const float f = l[r] == 0.f ? 0.f : 1.f / l[r];
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) {
+                        const float y[2] = {o[j][2 * r], o[j][2 * r + 1]};
+                        store_row<2>(p, u.rr.r0 + new_row[r], u.head * p.group + x % p.group, 8 * j + 2 * t, y, f);
+                    }
+                } else {
+                    float *to = part + r * 8 * (D + 4);
+#pragma unroll
+                    for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2 *>(to + 8 * j + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
+                    if (t == 0) to[D] = ref[r], to[D + 1] = l[r];
+                }
+            }
+            run.g += t1 - t0;
         }
-        run.g += t1 - t0;
     }
 }
 
@@ -828,26 +1193,32 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
 
             // scores of row t, without its factor
             float2 sv[NP];
-#pragma unroll
-            for (int pg = 0; pg < NP; ++pg) {
-                float c[4];
+            {
+                float c[NP][4];  // a chain of products a page, in turn
 #pragma unroll
                 for (int ch = 0; ch < kChunks; ++ch) {
-                    const uint8_t *from = st + pg * S::kBlock + mine * D + ch * 64 + t * 16;
-                    const uint4 w0 = *reinterpret_cast<const uint4 *>(from), w1 = *reinterpret_cast<const uint4 *>(from + 8 * D);
-                    const uint32_t a_w[4] = {w0.x, w0.y, w0.z, w0.w}, b_w[4] = {w1.x, w1.y, w1.z, w1.w};
+                    uint4 w0[NP], w1[NP];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        uint32_t a0, a1, a2, a3;
-                        codes_f16<FORMAT>(a_w[j], a0, a2);
-                        codes_f16<FORMAT>(b_w[j], a1, a3);
-                        if (ch == 0 && j == 0)
-                            mma16816_0(c, a0, a1, a2, a3, qf[0][0], qf[0][1]);
-                        else
-                            mma16816(c, a0, a1, a2, a3, qf[ch * 4 + j][0], qf[ch * 4 + j][1]);
+                    for (int pg = 0; pg < NP; ++pg) {
+                        const uint8_t *from = st + pg * S::kBlock + mine * D + ch * 64 + t * 16;
+                        w0[pg] = *reinterpret_cast<const uint4 *>(from), w1[pg] = *reinterpret_cast<const uint4 *>(from + 8 * D);
                     }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int pg = 0; pg < NP; ++pg) {
+                            uint32_t a0, a1, a2, a3;
+                            codes_f16<FORMAT>(j == 0 ? w0[pg].x : j == 1 ? w0[pg].y : j == 2 ? w0[pg].z : w0[pg].w, a0, a2);
+                            codes_f16<FORMAT>(j == 0 ? w1[pg].x : j == 1 ? w1[pg].y : j == 2 ? w1[pg].z : w1[pg].w, a1, a3);
+                            if (ch == 0 && j == 0)
+                                mma16816_0(c[pg], a0, a1, a2, a3, qf[0][0], qf[0][1]);
+                            else
+                                mma16816(c[pg], a0, a1, a2, a3, qf[ch * 4 + j][0], qf[ch * 4 + j][1]);
+                        }
                 }
-                sv[pg] = mul2(make_float2(c[0] + c[1], c[2] + c[3]), make_float2(sc[pg * 16 + mine], sc[pg * 16 + mine + 8]));
+#pragma unroll
+                for (int pg = 0; pg < NP; ++pg)
+                    sv[pg] = mul2(make_float2(c[pg][0] + c[pg][1], c[pg][2] + c[pg][3]), make_float2(sc[pg * 16 + mine], sc[pg * 16 + mine + 8]));
             }
             uint32_t seen = 0;  // bit: 2 page + (0 or 1)
             if (!whole) {

@@ -109,38 +109,56 @@ cudaError_t launch_read(ReadOp a, cudaStream_t st) {
 
 // ---- attention ---------------------------------------------------------------------------
 
-size_t round256(size_t n) { return (n + 255) / 256 * 256; }
-size_t plan_bytes() { return round256(sizeof(uint32_t) * (2 * kAk8MaxSeqs + 1)); }
 
 // The kernel of a call: which form, and what it needs.
 struct AttnForm {
-    void (*kernel)(AttnKv8), (*direct)(AttnKv8);
-    int warps, ring, tile_rows;
+    void (*kernel)(AttnKv8);
+    int warps, ctas, ring, tile_rows;  // ctas: of an SM
+    int runs;                          // warps or CTAs that take a run each; 0: a CTA has a whole unit (one launch)
 };
 
-template <int D, int FORMAT>
-AttnForm attn_form(int type, int64_t rows_per_unit) {
-    if (rows_per_unit <= 4)
-        return {k_attn_kv8_few<D, FORMAT, false>, k_attn_kv8_few<D, FORMAT, true>, Ak8Few<D>::kWarps, Ak8Few<D>::kRing, 4};
+template <int D, int FORMAT, int MODE>
+AttnForm attn_rows(int64_t rows_per_unit, bool direct) {
     using S = Ak8Shape<D>;
-    if (type == MOSSGPU_BF16) return {k_attn_kv8<D, FORMAT, false, false>, k_attn_kv8<D, FORMAT, false, true>, S::kWarps, S::kRing, 16};
-    return {k_attn_kv8<D, FORMAT, true, false>, k_attn_kv8<D, FORMAT, true, true>, S::kWarps, S::kRing, 8};
+    using B = Ak8Block<D>;
+    constexpr int kRows = Rows<D, MODE>::kRows;
+    if (direct) return {k_attn_kv8<D, FORMAT, MODE, true>, S::kWarps, 1, S::kRing, kRows, 0};
+    if (rows_per_unit <= kRows) return {k_attn_kv8<D, FORMAT, MODE, false>, S::kWarps, 1, S::kRing, kRows, kNumSMs * S::kWarps};
+    return {k_attn_kv8_block<D, FORMAT, MODE>, B::kWarps, B::kCtas, B::kRing, B::kWarps * kRows, kNumSMs * B::kCtas};
+}
+
+template <int D, int FORMAT>
+AttnForm attn_form(int type, int64_t rows_per_unit, int64_t rows, int n_seqs, int kv_heads, int pages) {
+    // A CTA a unit where they fit the machine at once and no warp gets long: one launch.  (Tiles are 32 positions.)
+    const auto direct = [&](int tile_rows, int warps) { return (rows / tile_rows + n_seqs) * kv_heads <= kNumSMs && pages <= 2 * 8 * warps; };
+    if (rows_per_unit <= 4) {
+        using S = Ak8Few<D>;
+        if (direct(4, S::kWarps)) return {k_attn_kv8_few<D, FORMAT, true>, S::kWarps, 1, S::kRing, 4, 0};
+        return {k_attn_kv8_few<D, FORMAT, false>, S::kWarps, 1, S::kRing, 4, kNumSMs * S::kWarps};
+    }
+    const bool one = direct(type == MOSSGPU_BF16 ? 16 : 8, Ak8Shape<D>::kWarps);
+    if (type != MOSSGPU_BF16) return attn_rows<D, FORMAT, kSplit>(rows_per_unit, one);
+    return attn_rows<D, FORMAT, kHalf>(rows_per_unit, one);
 }
 
 // Mean query rows of a sequence and kv head decide: the forms differ in speed, not in what they can do.
-AttnForm attn_form(int head_dim, int format, int type, int64_t rows, int n_seqs, int group) {
+AttnForm attn_form(const mossgpu_kv8_cache &c, int type, int64_t rows, int n_seqs, int group) {
     const int64_t per_unit = (rows + n_seqs - 1) / n_seqs * group;
-    if (head_dim == 64)
-        return format == MOSSGPU_KV_INT8 ? attn_form<64, MOSSGPU_KV_INT8>(type, per_unit) : attn_form<64, MOSSGPU_KV_E4M3>(type, per_unit);
-    return format == MOSSGPU_KV_INT8 ? attn_form<128, MOSSGPU_KV_INT8>(type, per_unit) : attn_form<128, MOSSGPU_KV_E4M3>(type, per_unit);
+    const auto form = c.head_dim == 64 ? (c.format == MOSSGPU_KV_INT8 ? attn_form<64, MOSSGPU_KV_INT8> : attn_form<64, MOSSGPU_KV_E4M3>)
+                                       : (c.format == MOSSGPU_KV_INT8 ? attn_form<128, MOSSGPU_KV_INT8> : attn_form<128, MOSSGPU_KV_E4M3>);
+    return form(type, per_unit, rows * group, n_seqs, c.kv_heads, c.pages_per_slot);
 }
 
-// Enough for every form
-size_t workspace_of(int head_dim, int64_t rows_in_unit) {
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+size_t plan_bytes() { return round256(sizeof(uint32_t) * (2 * kAk8MaxSeqs + 1)); }
+
+// Enough for every form: two partials a run and head
+size_t workspace_of(int head_dim, int kv_heads, int64_t rows_in_unit) {
     const size_t row = size_t(head_dim + 4) * sizeof(float);
-    const int few = head_dim == 64 ? Ak8Few<64>::kWarps : Ak8Few<128>::kWarps, many = head_dim == 64 ? Ak8Shape<64>::kWarps : Ak8Shape<128>::kWarps;
-    const size_t rows = std::max<int64_t>(few * std::min<int64_t>(4, rows_in_unit), many * std::min<int64_t>(16, rows_in_unit));
-    return plan_bytes() + size_t(2) * kNumSMs * rows * row;
+    const int64_t few = kNumSMs * (head_dim == 64 ? Ak8Few<64>::kWarps : Ak8Few<128>::kWarps) * std::min<int64_t>(4, rows_in_unit);
+    const int64_t warp = kNumSMs * (head_dim == 64 ? Ak8Shape<64>::kWarps : Ak8Shape<128>::kWarps) * std::min<int64_t>(16, rows_in_unit);
+    const int64_t block = std::max<int64_t>(kNumSMs * Ak8Block<64>::kCtas, kv_heads) * std::min<int64_t>(64, rows_in_unit);
+    return plan_bytes() + 2 * size_t(std::max(few, std::max(warp, block))) * row;
 }
 
 }  // namespace
@@ -297,7 +315,7 @@ size_t mossgpu_attention_kv8_workspace_bytes(const mossgpu_kv8_cache *cache, int
     if (!cache || q_heads <= 0 || rows <= 0 || cache->kv_heads < 1 || q_heads % cache->kv_heads ||
         (cache->head_dim != 64 && cache->head_dim != 128))
         return 0;
-    return workspace_of(cache->head_dim, int64_t(rows) * (q_heads / cache->kv_heads));
+    return workspace_of(cache->head_dim, cache->kv_heads, int64_t(rows) * (q_heads / cache->kv_heads));
 }
 
 int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *seqs, const mossgpu_attention_kv8_args *args,
@@ -325,7 +343,7 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
         return op_errorf("%s: the strides of out make its heads overlap", who);
     if (g.q == g.out) return op_errorf("%s: out must not be q", who);
     const int group = g.q_heads / cache->kv_heads;
-    const AttnForm f = attn_form(cache->head_dim, cache->format, g.type, seqs->rows, seqs->n_seqs, group);
+    const AttnForm f = attn_form(*cache, g.type, seqs->rows, seqs->n_seqs, group);
     const int64_t jobs = int64_t(seqs->rows) * g.q_heads;
     if (jobs > (int64_t(1) << 33)) return op_errorf("%s: rows * q_heads is above 2^33", who);
     // the plan counts tiles in 32 bits
@@ -339,29 +357,26 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     p.seqs = *seqs;
     p.a = g;
     p.group = group;
-    p.runs = kNumSMs * f.warps / cache->kv_heads;
+    p.runs = std::max(1, f.runs / cache->kv_heads);
     p.tile_rows = f.tile_rows;
     p.part_rows = int(std::min<int64_t>(f.tile_rows, int64_t(seqs->rows) * group));
-    // A CTA a unit where they fit the machine at once and no warp gets long: one launch.  (Tiles are 32 positions.)
     const int64_t units = (int64_t(seqs->rows) * group / f.tile_rows + seqs->n_seqs) * cache->kv_heads;
-    const bool direct = units <= kNumSMs && cache->pages_per_slot <= 2 * 8 * f.warps;
     p.vec_q = vec_ok(g.q, g.q_row_stride, g.q_head_stride, g.type);
     p.vec_out = vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
     p.plan = static_cast<uint32_t *>(g.workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(g.workspace) + plan_bytes());
     p.status = status;
-    const auto kernel = direct ? f.direct : f.kernel;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(f.kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          f.ring + int(sizeof(uint32_t)) * (kAk8MaxSeqs + 1));
     if (e != cudaSuccess) return op_errorf("%s: cudaFuncSetAttribute: %s", who, cudaGetErrorString(e));
     cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(direct ? unsigned(units) : unsigned(kNumSMs));
+    cfg.gridDim = dim3(f.runs ? unsigned(kNumSMs * f.ctas) : unsigned(units));
     cfg.blockDim = dim3(unsigned(f.warps) * 32);
     cfg.dynamicSmemBytes = size_t(f.ring) + sizeof(uint32_t) * (seqs->n_seqs + 1);
     cfg.stream = static_cast<cudaStream_t>(cuda_stream);
-    e = cudaLaunchKernelEx(&cfg, kernel, p);
+    e = cudaLaunchKernelEx(&cfg, f.kernel, p);
     if (e != cudaSuccess) return op_errorf("%s launch: %s", who, cudaGetErrorString(e));
-    if (direct) return 0;
+    if (f.runs == 0) return 0;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
