@@ -65,39 +65,44 @@ bool distinct(int rows, int heads, int head_dim, int64_t row, int64_t head) {
 }
 
 // Warps that share a row (or a few rows) of `passes` passes: one where the rows alone fill the
-// machine twice over, as many as there are passes where they do not.
+// machine, as many as there are passes where they do not.
 int warps_for(int64_t rows, int passes) {
-    const int64_t want = int64_t(kNumSMs) * 64;
+    const int64_t want = int64_t(kNumSMs) * 32;
     return int(std::max<int64_t>(1, std::min<int64_t>(passes, (want + rows - 1) / rows)));
 }
 unsigned blocks_for(int64_t warps) { return unsigned((warps + kRowThreads / 32 - 1) / (kRowThreads / 32)); }
 
-template <typename T>
+template <typename T, int LAYOUT>
 cudaError_t launch_rope(RowOp a, cudaStream_t st) {
-    const int lanes = a.head_dim <= 32 ? 4 : a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32;
-    const int items = a.heads[0] + a.heads[1] + a.heads[2];
-    a.row_warps = warps_for(a.rows, (items * lanes + 31) / 32);
+    const int lanes = a.head_dim <= 32 ? 4 : a.head_dim <= 64 ? 8 : a.head_dim <= 128 ? 16 : 32, heads = 32 / lanes;
+    a.row_warps = warps_for(a.rows, (a.heads[0] + heads - 1) / heads + 2 * ((a.heads[1] + heads - 1) / heads));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(blocks_for(int64_t(a.rows) * a.row_warps));
     cfg.blockDim = dim3(kRowThreads);
     cfg.stream = st;
-    if (lanes == 4) return cudaLaunchKernelEx(&cfg, k_rope_append<T, 4>, a);
-    if (lanes == 8) return cudaLaunchKernelEx(&cfg, k_rope_append<T, 8>, a);
-    if (lanes == 16) return cudaLaunchKernelEx(&cfg, k_rope_append<T, 16>, a);
-    return cudaLaunchKernelEx(&cfg, k_rope_append<T, 32>, a);
+    if (a.heads[1] > 0)
+        return lanes == 8 ? cudaLaunchKernelEx(&cfg, k_rope_append<T, 8, LAYOUT, true>, a)
+                          : cudaLaunchKernelEx(&cfg, k_rope_append<T, 16, LAYOUT, true>, a);
+    if (lanes == 4) return cudaLaunchKernelEx(&cfg, k_rope_append<T, 4, LAYOUT, false>, a);
+    if (lanes == 8) return cudaLaunchKernelEx(&cfg, k_rope_append<T, 8, LAYOUT, false>, a);
+    if (lanes == 16) return cudaLaunchKernelEx(&cfg, k_rope_append<T, 16, LAYOUT, false>, a);
+    return cudaLaunchKernelEx(&cfg, k_rope_append<T, 32, LAYOUT, false>, a);
 }
 
-int run_rope(const RowOp &a, int type, void *stream, const char *who) {
+int run_rope(const RowOp &a, int type, bool vec, void *stream, const char *who) {
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = type == MOSSGPU_F32   ? launch_rope<float>(a, st)
-                          : type == MOSSGPU_F16 ? launch_rope<__half>(a, st)
-                                                : launch_rope<__nv_bfloat16>(a, st);
+    const int layout = !vec ? kAny : a.rope.rotary_dim == 0 || a.rope.interleaved ? kPairs : a.rope.rotary_dim % 8 == 0 ? kHalves : kAny;
+    const auto of = [&](auto zero) {
+        using T = decltype(zero);
+        return layout == kPairs ? launch_rope<T, kPairs>(a, st) : layout == kHalves ? launch_rope<T, kHalves>(a, st) : launch_rope<T, kAny>(a, st);
+    };
+    const cudaError_t e = type == MOSSGPU_F32 ? of(float()) : type == MOSSGPU_F16 ? of(__half()) : of(__nv_bfloat16());
     return e == cudaSuccess ? 0 : op_errorf("%s launch: %s", who, cudaGetErrorString(e));
 }
 
 template <typename T>
 cudaError_t launch_read(ReadOp a, cudaStream_t st) {
-    const int rows = a.cache.head_dim == 64 ? 8 : 4;  // of a warp
+    const int rows = a.cache.head_dim == 64 ? 16 : 8;  // of a warp
     const int64_t groups = (int64_t(a.seqs.rows) + rows - 1) / rows;
     a.row_warps = warps_for(groups, 2 * a.cache.kv_heads);
     cudaLaunchConfig_t cfg{};
@@ -225,13 +230,12 @@ int mossgpu_rope_rotate(const mossgpu_rope *rope, const mossgpu_rope_args *args,
     a.out_row_stride = g.out_row_stride, a.out_head_stride = g.out_head_stride;
     a.pos = g.pos;
     a.heads[0] = g.heads;
-    a.vec[0] = vec_ok(g.x, g.x_row_stride, g.x_head_stride, g.type);
-    a.vec_out = vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
+    const bool vec = vec_ok(g.x, g.x_row_stride, g.x_head_stride, g.type) && vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
     a.rows = g.rows;
     a.head_dim = g.head_dim;
     a.inverse = g.inverse;
     a.status = status;
-    return run_rope(a, g.type, cuda_stream, who);
+    return run_rope(a, g.type, vec, cuda_stream, who);
 }
 
 int mossgpu_kv8_append(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *seqs, const mossgpu_rope *rope,
@@ -268,13 +272,13 @@ int mossgpu_kv8_append(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *
     a.out_row_stride = g.q_out_row_stride, a.out_head_stride = g.q_out_head_stride;
     a.pos = g.pos;
     a.heads[0] = g.q ? g.q_heads : 0;
-    a.heads[1] = a.heads[2] = cache->kv_heads;
-    for (int i = 0; i < 3; ++i) a.vec[i] = vec_ok(a.src[i], a.row_stride[i], a.head_stride[i], g.type);
-    a.vec_out = vec_ok(g.q_out, g.q_out_row_stride, g.q_out_head_stride, g.type);
+    a.heads[1] = cache->kv_heads;
+    bool vec = !g.q || vec_ok(g.q_out, g.q_out_row_stride, g.q_out_head_stride, g.type);
+    for (int i = g.q ? 0 : 1; i < 3; ++i) vec = vec && vec_ok(a.src[i], a.row_stride[i], a.head_stride[i], g.type);
     a.rows = seqs->rows;
     a.head_dim = cache->head_dim;
     a.status = status;
-    return run_rope(a, g.type, cuda_stream, who);
+    return run_rope(a, g.type, vec, cuda_stream, who);
 }
 
 int mossgpu_kv8_read(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *seqs, const mossgpu_kv8_read_args *args,

@@ -19,6 +19,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <float.h>
 #include <math.h>
 #include <string.h>
 
@@ -200,49 +201,72 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT
         // ---- candidates: few threads have any
         const bool few = bound == -INFINITY;  // fewer than k groups hold anything: every finite logit, and the first ids
         if (mine >= bound) {
+            const float least = few ? -FLT_MAX : bound;
+            constexpr int kWords = (NV * VE + 31) / 32;
+            uint32_t in[kWords];
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                uint32_t in = 0;
+            for (int w = 0; w < kWords; ++w) in[w] = 0;
+#pragma unroll
+            for (int v = 0; v < NV; ++v)
 #pragma unroll
                 for (int i = 0; i < VE / 2; ++i) {
                     const float2 f = pair_of<T>(x[v], i);
-                    if (few ? f.x > bound : f.x >= bound) in |= 1u << (2 * i);
-                    if (few ? f.y > bound : f.y >= bound) in |= 2u << (2 * i);
+                    const int bit = (v * VE + 2 * i) % 32;
+                    if (f.x >= least) in[(v * VE) / 32] |= 1u << bit;
+                    if (f.y >= least) in[(v * VE) / 32] |= 2u << bit;
                 }
-                const int e0 = id_of(v, 0);
-                if (few && e0 < a.top_k) {
+            if (few) {
+#pragma unroll
+                for (int v = 0; v < NV; ++v) {
+                    const int e0 = id_of(v, 0);
+                    if (e0 >= a.top_k) continue;
                     for (int i = 0; i < VE; ++i)
-                        if (e0 + i >= 0 && e0 + i < a.top_k) in |= 1u << i;
-                }
-                for (; in; in &= in - 1) {
-                    const int id = e0 + __ffs(in) - 1, at = atomicAdd(&n_cand, 1);
-                    if (at < kCandidates) cand[at] = order_key(float(x_row[id]), id);
+                        if (e0 + i >= 0 && e0 + i < a.top_k) in[(v * VE) / 32] |= 1u << ((v * VE) % 32 + i);
                 }
             }
+#pragma unroll
+            for (int w = 0; w < kWords; ++w)
+                for (; in[w]; in[w] &= in[w] - 1) {
+                    const int e = w * 32 + __ffs(in[w]) - 1, id = id_of(e / VE, e % VE), at = atomicAdd(&n_cand, 1);
+                    if (at < kCandidates) cand[at] = order_key(float(x_row[id]), id);
+                }
         }
     }
 
     // ---- sums
-    float2 z = make_float2(0.f, 0.f), s = z;
+    float z = 0.f, s = 0.f;
     const float c = 1.4426950408889634f / a.temperature;
-    const float2 c2 = make_float2(c, c), off = make_float2(-top, -top);
+    // (x - M) c as one operation where that cannot pass the range of fp32: its terms are relative to what
+    // M c rounds to, which the sums are corrected for
+    const float off = -top * c;
+    float miss = 0.f;  // by how much they are too large
+    if (fabsf(off) < 1e30f) {
+        miss = fmaf(top, c, off);
 #pragma unroll
-    for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v)
 #pragma unroll
-        for (int i = 0; i < VE / 2; ++i) {
-            float2 t = mul2(add2(pair_of<T>(x[v], i), off), c2), e;
-            t.x = fmaxf(t.x, -200.f), t.y = fmaxf(t.y, -200.f);  // 2^-200 is 0, and 0 * infinity stays out of the sum
-            e.x = ex2(t.x), e.y = ex2(t.y);
-            z = add2(z, e);
-            s = fma2(e, t, s);
+            for (int i = 0; i < VE / 2; ++i) {
+                const float2 f = pair_of<T>(x[v], i);
+                const float t0 = fmaxf(fmaf(f.x, c, off), -200.f), t1 = fmaxf(fmaf(f.y, c, off), -200.f);
+                const float e0 = ex2(t0), e1 = ex2(t1);  // 2^-200 is 0, and 0 * infinity stays out of the sum
+                z += e0, s = fmaf(e0, t0, s);
+                z += e1, s = fmaf(e1, t1, s);
+            }
+    } else {
+#pragma unroll 1
+        for (int v = 0; v < NV * VE; ++v) {
+            const int id = id_of(v / VE, v % VE);
+            if (id < 0 || id >= a.vocab) continue;
+            const float t = fmaxf((float(x_row[id]) - top) * c, -200.f), e = ex2(t);
+            z += e, s = fmaf(e, t, s);
         }
-    z.x += z.y, s.x += s.y;
+    }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
-        z.x += __shfl_xor_sync(0xffffffffu, z.x, o);
-        s.x += __shfl_xor_sync(0xffffffffu, s.x, o);
+        z += __shfl_xor_sync(0xffffffffu, z, o);
+        s += __shfl_xor_sync(0xffffffffu, s, o);
     }
-    if (lane == 0) warp_sums[tid >> 5] = make_float2(z.x, s.x);
+    if (lane == 0) warp_sums[tid >> 5] = make_float2(z, s);
     __syncthreads();
     int n = n_cand;
     if (a.top_k > 0 && (!sound || n > kCandidates)) n = select_exact<T, NT>(x_row, a.vocab, a.top_k, NV, id_of, &n_cand, cand);
@@ -266,7 +290,11 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT
             t.x += __shfl_xor_sync(0xffffffffu, t.x, o);
             t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
         }
-        if (tid == 0) mine_part->top = top, mine_part->z = t.x, mine_part->s = t.y, mine_part->count = min(n, a.top_k);
+        if (tid == 0) {
+            const float f = fmaf(-miss, kLpLn2, 1.f);  // 2^-miss
+            mine_part->top = top, mine_part->z = t.x * f, mine_part->s = fmaf(-miss, t.x, t.y) * f;
+            mine_part->count = min(n, a.top_k);
+        }
     }
     if (ctas > 1) {
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");

@@ -3,8 +3,7 @@
 // All three are bound by HBM: an element is read once and written once, with a few instructions
 // between.  Work goes to independent warps (no CTA barriers).  In k_rope_append LPH lanes (a power
 // of two) share a head, 8 elements a lane, and a warp takes several heads of one row: a lane has the
-// same columns in all of them, so its cosines and sines are computed once.  The loads of kAhead
-// passes are in flight together, the first of them issued before the row's place is looked up.
+// same columns in all of them, so its cosines and sines are computed once.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -93,60 +92,106 @@ __device__ __forceinline__ float2 rope_angle(int pos, uint64_t step, float magni
     return make_float2(c * magnitude, inverse ? -s * magnitude : s * magnitude);
 }
 
-// A lane's share of the rotation: elements base .. base + 7 of every head.  Interleaved, it holds
-// both members of four pairs.  In the half layout the other member is rot / 2 elements away: in one
-// other lane where rot is a multiple of 16 (shuffles), anywhere otherwise (through `stage`, 256
-// floats of this warp).  The sine has its sign: y = x cos + partner sin.
-struct LaneRope {
-    float c[8], s[8];
-    int turn;   // 0: nothing of this lane turns, 1: all, 2: some elements (mask)
-    uint32_t mask;
+// A lane's share of a head is two chunks of 4 elements, at `first` and `second`.  kPairs: interleaved
+// pairs (2i, 2i + 1) inside the chunks, which lie behind one another: one 16-byte vector in 16-bit types.
+// kHalves: the half layout with a rotary_dim that is a multiple of 8; lane j < rotary_dim / 8 has elements
+// 4j.. and their partners at rotary_dim / 2 + 4j.., the lanes behind it 8 neighbouring ones, so that no
+// element has its partner in another lane.  Both move 8 or 16 bytes at a time.  kAny: either layout, any
+// rotary_dim and alignment: element by element, partners by way of shared memory.
+constexpr int kPairs = 0, kHalves = 1, kAny = 2;
+
+// The two chunks of a lane, as they lie in memory.
+template <typename T>
+struct Raw8 {
+    uint2 w[sizeof(T)];
 };
-__device__ __forceinline__ LaneRope lane_rope(const mossgpu_rope &r, int pos, int base, bool inverse) {
-    LaneRope t;
-    t.mask = 0;
-    const int half = r.rotary_dim / 2;
-    if (r.interleaved) {
+template <typename T, int LAYOUT>
+__device__ __forceinline__ Raw8<T> raw8(const T *p, int first, int second) {
+    Raw8<T> r;
+    if constexpr (LAYOUT == kAny) {
+        T e[8];
 #pragma unroll
-        for (int m = 0; m < 4; ++m) {
-            t.c[2 * m] = t.c[2 * m + 1] = 1.f, t.s[2 * m] = t.s[2 * m + 1] = 0.f;
-            if (base + 2 * m < r.rotary_dim) {
-                const float2 v = rope_angle(pos, __ldg(r.steps + base / 2 + m), r.magnitude, inverse);
-                t.c[2 * m] = t.c[2 * m + 1] = v.x;
-                t.s[2 * m] = -v.y, t.s[2 * m + 1] = v.y;
-                t.mask |= 3u << (2 * m);
-            }
-        }
+        for (int i = 0; i < 4; ++i) e[i] = p[first + i], e[4 + i] = p[second + i];
+        memcpy(&r, e, sizeof(r));
+    } else if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<uint4 *>(&r)[0] = *reinterpret_cast<const uint4 *>(p + first);
+        reinterpret_cast<uint4 *>(&r)[1] = *reinterpret_cast<const uint4 *>(p + second);
+    } else if constexpr (LAYOUT == kPairs) {
+        *reinterpret_cast<uint4 *>(&r) = *reinterpret_cast<const uint4 *>(p + first);
     } else {
+        r.w[0] = *reinterpret_cast<const uint2 *>(p + first);
+        r.w[1] = *reinterpret_cast<const uint2 *>(p + second);
+    }
+    return r;
+}
+template <typename T, int LAYOUT>
+__device__ __forceinline__ void put8(T *p, int first, int second, const float (&x)[8]) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = T(x[i]);
+    Raw8<T> r;
+    memcpy(&r, e, sizeof(r));
+    if constexpr (LAYOUT == kAny) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[first + i] = e[i], p[second + i] = e[4 + i];
+    } else if constexpr (sizeof(T) == 4) {
+        *reinterpret_cast<uint4 *>(p + first) = reinterpret_cast<uint4 *>(&r)[0];
+        *reinterpret_cast<uint4 *>(p + second) = reinterpret_cast<uint4 *>(&r)[1];
+    } else if constexpr (LAYOUT == kPairs) {
+        *reinterpret_cast<uint4 *>(p + first) = *reinterpret_cast<uint4 *>(&r);
+    } else {
+        *reinterpret_cast<uint2 *>(p + first) = r.w[0];
+        *reinterpret_cast<uint2 *>(p + second) = r.w[1];
+    }
+}
+template <typename T>
+__device__ __forceinline__ void raw_f32(const Raw8<T> &r, float (&x)[8]) {
+    T e[8];
+    memcpy(e, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = float(e[i]);
+}
+
+template <int LAYOUT>
+struct LaneRope {
+    float c[LAYOUT == kAny ? 8 : 4], s[LAYOUT == kAny ? 8 : 4];  // of pairs; kAny: of elements, the sine with its sign
+    uint32_t mask;                                               // what turns
+};
+template <int LAYOUT>
+__device__ __forceinline__ LaneRope<LAYOUT> lane_rope(const mossgpu_rope &r, int pos, int lane_in_head, bool inverse) {
+    LaneRope<LAYOUT> t;
+    t.mask = 0;
+    if constexpr (LAYOUT == kAny) {
+        const int half = r.rotary_dim / 2;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const int e = base + j;
-            t.c[j] = 1.f, t.s[j] = 0.f;
+            const int e = lane_in_head * 8 + j;
             if (e < r.rotary_dim) {
-                const bool first = e < half;
-                const float2 v = rope_angle(pos, __ldg(r.steps + (first ? e : e - half)), r.magnitude, inverse);
+                const bool first = r.interleaved ? !(e & 1) : e < half;
+                const float2 v = rope_angle(pos, __ldg(r.steps + (r.interleaved ? e / 2 : first ? e : e - half)), r.magnitude, inverse);
                 t.c[j] = v.x, t.s[j] = first ? -v.y : v.y;
                 t.mask |= 1u << j;
             }
         }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int i = lane_in_head * 4 + k;  // the pair, in both layouts
+            if (2 * i < r.rotary_dim) {
+                const float2 v = rope_angle(pos, __ldg(r.steps + i), r.magnitude, inverse);
+                t.c[k] = v.x, t.s[k] = v.y;
+                t.mask |= 1u << k;
+            }
+        }
     }
-    t.turn = t.mask == 0 ? 0 : t.mask == 0xffu ? 1 : 2;
     return t;
 }
-// All lanes of the warp call it; `on`: this lane's head turns.
-__device__ __forceinline__ void rope_turn(float (&x)[8], const mossgpu_rope &r, const LaneRope &t, bool on, int base, float *stage,
-                                          int lph) {
-    float p[8];
-    if (r.interleaved) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = x[j ^ 1];
-    } else if (r.rotary_dim % 16 == 0) {
-        const int lane = threadIdx.x & 31, d = r.rotary_dim / 16;
-        const int from = t.turn ? (base < r.rotary_dim / 2 ? lane + d : lane - d) : lane;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) p[j] = __shfl_sync(0xffffffffu, x[j], from);
-    } else {
-        const int lane = threadIdx.x & 31, half = r.rotary_dim / 2;
+// x[0..3] and x[4..7]: the two chunks.  Elements that do not turn stay as they are, whatever their bits.
+// All lanes of the warp call the kAny form; `stage`: 256 floats of this warp, lph lanes a head.
+template <int LAYOUT>
+__device__ __forceinline__ void rope_turn(float (&x)[8], const LaneRope<LAYOUT> &t, const mossgpu_rope &r, float *stage, int lph) {
+    if constexpr (LAYOUT == kAny) {
+        const int lane = threadIdx.x & 31, half = r.rotary_dim / 2, base = (lane & (lph - 1)) * 8;
         const float *head = stage + (lane & ~(lph - 1)) * 8;
         __syncwarp();
         reinterpret_cast<float4 *>(stage + lane * 8)[0] = make_float4(x[0], x[1], x[2], x[3]);
@@ -155,14 +200,26 @@ __device__ __forceinline__ void rope_turn(float (&x)[8], const mossgpu_rope &r, 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int e = base + j;
-            p[j] = e < r.rotary_dim ? head[e < half ? e + half : e - half] : 0.f;
+            if (t.mask >> j & 1u) x[j] = x[j] * t.c[j] + head[r.interleaved ? e ^ 1 : e < half ? e + half : e - half] * t.s[j];
         }
-    }
-    if (on && t.turn) {
-        // elements past rotary_dim stay as they are, whatever their bits
+    } else if (t.mask == 0xfu) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            if (t.turn == 1 || (t.mask >> j & 1u)) x[j] = x[j] * t.c[j] + p[j] * t.s[j];
+        for (int k = 0; k < 4; ++k) {
+            float &a = x[LAYOUT == kPairs ? 2 * k : k], &b = x[LAYOUT == kPairs ? 2 * k + 1 : k + 4];
+            const float ya = a * t.c[k] - b * t.s[k];
+            b = b * t.c[k] + a * t.s[k];
+            a = ya;
+        }
+    } else if (t.mask) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            float &a = x[LAYOUT == kPairs ? 2 * k : k], &b = x[LAYOUT == kPairs ? 2 * k + 1 : k + 4];
+            if (t.mask >> k & 1u) {
+                const float ya = a * t.c[k] - b * t.s[k];
+                b = b * t.c[k] + a * t.s[k];
+                a = ya;
+            }
+        }
     }
 }
 
@@ -210,8 +267,7 @@ struct RowOp {
     void *q_out;             // may be src[0]
     int64_t row_stride[3], head_stride[3], out_row_stride, out_head_stride;
     const int32_t *pos;
-    int heads[3];
-    int vec[3], vec_out;
+    int heads[2];            // of q, of k and v
     int rows, row_warps;     // warps that share a row
     int head_dim, inverse;
     int *status;
@@ -239,65 +295,24 @@ __device__ __forceinline__ bool row_place(const mossgpu_kv8_cache &c, const moss
     return true;
 }
 
-template <typename T>
-struct Raw8 {  // 8 elements as they lie in memory
-    uint4 w[sizeof(T) / 2];
-};
-template <typename T>
-__device__ __forceinline__ Raw8<T> raw8(const T *p, bool vec) {
-    Raw8<T> r;
-    if (vec) {
-#pragma unroll
-        for (int i = 0; i < int(sizeof(T) / 2); ++i) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
-    } else {
-        T e[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) e[i] = p[i];
-        memcpy(&r, e, sizeof(r));
-    }
-    return r;
-}
-template <typename T>
-__device__ __forceinline__ void raw_f32(const Raw8<T> &r, float (&x)[8]) {
-    T e[8];
-    memcpy(e, &r, sizeof(r));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = float(e[i]);
-}
-
-// q (and k) of a row turned, k and v quantised into the cache.
-template <typename T, int LPH>
-__global__ void __launch_bounds__(kRowThreads) k_rope_append(const __grid_constant__ RowOp a) {
+// q (and, with KV, k) of a row turned, k and v quantised into the cache.  A pass is 32 / LPH heads of one
+// tensor; the row's warps take the passes of q, k and v in turn.
+template <typename T, int LPH, int LAYOUT, bool KV>
+__global__ void __launch_bounds__(kRowThreads, 3) k_rope_append(const __grid_constant__ RowOp a) {
     constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // passes whose loads are in flight together
     constexpr int kHeads = 32 / LPH;                // heads a pass
-    __shared__ __align__(16) float stage[kRowThreads * 8];
+    __shared__ __align__(16) float stage[LAYOUT == kAny ? kRowThreads * 8 : 4];
     const int lane = threadIdx.x & 31;
     const uint32_t job = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5);
     const uint32_t job_row = job / uint32_t(a.row_warps);
     if (job_row >= uint32_t(a.rows)) return;
     const int row = int(job_row), part = int(job - job_row * uint32_t(a.row_warps));
-    const int base = (lane & (LPH - 1)) * 8, D = a.head_dim, hq = a.heads[0], hk = hq + a.heads[1], items = hk + a.heads[2];
-    const auto head_of = [&](int it, int &kind) {
-        kind = it < hq ? 0 : it < hk ? 1 : 2;
-        return kind == 0 ? it : kind == 1 ? it - hq : it - hk;
-    };
-    const int step = a.row_warps * kHeads;  // this warp's passes: part * kHeads, + step, ...
-    Raw8<T> raw[kAhead];
-    const auto fetch = [&](int it0) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            const int it = it0 + u * step + lane / LPH;
-            int kind;
-            const int h = head_of(it, kind);
-            if (it < items && base < D)
-                raw[u] = raw8(static_cast<const T *>(a.src[kind]) + row * a.row_stride[kind] + h * a.head_stride[kind] + base,
-                              a.vec[kind] != 0);
-        }
-    };
-    int it0 = part * kHeads;
-    fetch(it0);
+    const int in_head = lane & (LPH - 1), sub = lane / LPH, D = a.head_dim, rot = a.rope.rotary_dim;
+    const bool here = in_head * 8 < D;
+    int first = in_head * 8, second = first + 4;
+    if (LAYOUT == kHalves && first < rot) first = in_head * 4, second = first + rot / 2;
     int pos = 0, page = -1, off = 0;
-    if (a.seqs.n_seqs > 0) {
+    if (KV) {
         RowPlace w;
         int status = 0;
         const int s = warp_upper_bound(a.seqs.row_start, a.seqs.n_seqs, row) - 1;
@@ -309,40 +324,63 @@ __global__ void __launch_bounds__(kRowThreads) k_rope_append(const __grid_consta
     } else {
         pos = __ldg(a.pos + row);
     }
-    LaneRope turn;
-    const int rot = a.rope.rotary_dim;
-    if (rot > 0) turn = lane_rope(a.rope, pos, base, a.inverse != 0);
-    float *st = stage + (threadIdx.x & ~31u) * 8;
-    for (; it0 < items; it0 += kAhead * step) {
-        float x[kAhead][8];
+    LaneRope<LAYOUT> turn;
+    turn.mask = 0;
+    if (rot > 0) turn = lane_rope<LAYOUT>(a.rope, pos, in_head, a.inverse != 0);
+    float *st = LAYOUT == kAny ? stage + (threadIdx.x & ~31u) * 8 : stage;
+    // the heads of one tensor, from this warp's first pass on; use(head, live, x) for each
+    const auto run = [&](const void *src, int64_t row_stride, int64_t head_stride, int heads, int my_part, auto &&use) {
+        const int step = a.row_warps * kHeads;
+        const T *p = static_cast<const T *>(src) + row * row_stride + int64_t(my_part * kHeads + sub) * head_stride;
+        for (int h0 = my_part * kHeads; h0 < heads; h0 += kAhead * step) {
+            Raw8<T> raw[kAhead];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) raw_f32(raw[u], x[u]);
-        if (it0 + kAhead * step < items) fetch(it0 + kAhead * step);
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-            if (it0 + u * step >= items) break;  // the whole warp
-            const int it = it0 + u * step + lane / LPH;
-            int kind;
-            const int h = head_of(it, kind);
-            const bool live = it < items && base < D;
-            if (!live) {
-#pragma unroll
-                for (int j = 0; j < 8; ++j) x[u][j] = 0.f;
+            for (int u = 0; u < kAhead; ++u) {
+                if (here && h0 + u * step + sub < heads) raw[u] = raw8<T, LAYOUT>(p, first, second);
+                p += step * head_stride;
             }
-            if (rot > 0) rope_turn(x[u], a.rope, turn, kind < 2, base, st, LPH);
-            if (kind == 0 && live)
-                store8(static_cast<T *>(a.q_out) + row * a.out_row_stride + h * a.out_head_stride + base, a.vec_out != 0, x[u]);
-            if constexpr (LPH == 8 || LPH == 16) {  // head_dim 64, 128: the cache's
-                if (__any_sync(0xffffffffu, kind > 0 && live)) {
-                    float scale;
-                    const uint2 c = quantise8<LPH>(x[u], a.cache.format, &scale);
-                    if (live && kind > 0 && page >= 0) {
-                        const size_t cell = kv8_cell(a.cache, page, kind - 1, h, off);
-                        *reinterpret_cast<uint2 *>(static_cast<uint8_t *>(a.cache.codes) + cell * size_t(D) + base) = c;
-                        if (base == 0) a.cache.scales[cell] = scale;
-                    }
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (h0 + u * step >= heads) break;  // the whole warp
+                const int h = h0 + u * step + sub;
+                const bool live = here && h < heads;
+                float x[8];
+                raw_f32(raw[u], x);
+                use(h, live, x);
+            }
+        }
+    };
+    T *out_row = static_cast<T *>(a.q_out) + row * a.out_row_stride;
+    run(a.src[0], a.row_stride[0], a.head_stride[0], a.heads[0], part, [&](int h, bool live, float (&x)[8]) {
+        if (LAYOUT == kAny || live) rope_turn<LAYOUT>(x, turn, a.rope, st, LPH);
+        if (live) put8<T, LAYOUT>(out_row + h * a.out_head_stride, first, second, x);
+    });
+    if constexpr (KV) {
+        int before = (a.heads[0] + kHeads - 1) / kHeads;  // passes of the tensors before
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int my_part = (part + a.row_warps - before % a.row_warps) % a.row_warps;
+            run(a.src[1 + half], a.row_stride[1 + half], a.head_stride[1 + half], a.heads[1], my_part, [&](int h, bool live, float (&x)[8]) {
+                if (half == 0 && rot > 0 && (LAYOUT == kAny || live)) rope_turn<LAYOUT>(x, turn, a.rope, st, LPH);
+                if (!live) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = 0.f;
                 }
-            }
+                float scale;
+                const uint2 c = quantise8<LPH>(x, a.cache.format, &scale);
+                if (live && page >= 0) {
+                    const size_t cell = kv8_cell(a.cache, page, half, h, off);
+                    uint8_t *codes = static_cast<uint8_t *>(a.cache.codes) + cell * size_t(LPH * 8);
+                    if constexpr (LAYOUT == kHalves) {
+                        *reinterpret_cast<uint32_t *>(codes + first) = c.x;
+                        *reinterpret_cast<uint32_t *>(codes + second) = c.y;
+                    } else {
+                        *reinterpret_cast<uint2 *>(codes + first) = c;
+                    }
+                    if (in_head == 0) a.cache.scales[cell] = scale;
+                }
+            });
+            before += (a.heads[1] + kHeads - 1) / kHeads;
         }
     }
 }
@@ -379,48 +417,69 @@ __device__ __forceinline__ void dequantise8(uint32_t lo, uint32_t hi, int format
     }
 }
 
-// A warp takes kRows neighbouring rows, 16 codes a lane: positions of a page lie behind one another
-// for each head, so that a pass reads 512 contiguous bytes where the rows share a page.
+// A warp takes kSets times kRows neighbouring rows, 16 codes a lane: positions of a page lie behind one
+// another for each head, so that a load reads 512 contiguous bytes where the rows share a page.
 template <typename T, int D>
 __global__ void __launch_bounds__(kRowThreads) k_kv8_read(const __grid_constant__ ReadOp a) {
-    constexpr int kLanes = D / 16, kRows = 32 / kLanes, kAhead = 4;
+    constexpr int kLanes = D / 16, kRows = 32 / kLanes, kSets = 2, kAhead = 4;
     const int lane = threadIdx.x & 31;
     const uint32_t job = blockIdx.x * (kRowThreads / 32) + (threadIdx.x >> 5), group = job / uint32_t(a.row_warps);
-    const int64_t first = int64_t(group) * kRows;
+    const int64_t from = int64_t(group) * (kRows * kSets);
     const int part = int(job - group * uint32_t(a.row_warps));
-    if (first >= a.seqs.rows) return;
-    const int row = int(min(first + lane / kLanes, int64_t(a.seqs.rows) - 1));  // lanes past the end repeat the last row
-    int s = warp_upper_bound(a.seqs.row_start, a.seqs.n_seqs, int(first)) - 1;
-    // further rows may belong to later sequences: the last one that begins at or before the row
-    while (s + 1 < a.seqs.n_seqs && __ldg(a.seqs.row_start + s + 1) <= row) ++s;
-    RowPlace w;
-    int status = 0;
-    const bool owned = row_place(a.cache, a.seqs, s, row, w, &status);
-    op_report(a.status, status);
-    const bool live = owned && w.page >= 0;
+    if (from >= a.seqs.rows) return;
+    const int s0 = warp_upper_bound(a.seqs.row_start, a.seqs.n_seqs, int(from)) - 1;
     const int base = (lane & (kLanes - 1)) * 16, H = a.cache.kv_heads;
+    int row[kSets];
+    const uint8_t *codes[kSets];  // of the row's position in head 0 of K
+    const float *scales[kSets];
+#pragma unroll
+    for (int i = 0; i < kSets; ++i) {
+        row[i] = int(min(from + i * kRows + lane / kLanes, int64_t(a.seqs.rows) - 1));  // lanes past the end repeat the last row
+        int s = s0;
+        // further rows may belong to later sequences: the last one that begins at or before the row
+        while (s + 1 < a.seqs.n_seqs && __ldg(a.seqs.row_start + s + 1) <= row[i]) ++s;
+        RowPlace w;
+        int status = 0;
+        const bool owned = row_place(a.cache, a.seqs, s, row[i], w, &status);
+        op_report(a.status, status);
+        codes[i] = nullptr;
+        if (owned && w.page >= 0) {
+            const size_t cell = kv8_cell(a.cache, w.page, 0, 0, w.off);
+            codes[i] = static_cast<const uint8_t *>(a.cache.codes) + cell * D + base;
+            scales[i] = a.cache.scales + cell;
+        }
+    }
+    // item it < H: head it of K, else head it - H of V; they follow one another in the cache
     for (int it0 = part; it0 < 2 * H; it0 += kAhead * a.row_warps) {
-        uint4 c[kAhead];
-        float scale[kAhead];
+        uint4 c[kAhead][kSets];
+        float scale[kAhead][kSets];
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
-            const int it = it0 + u * a.row_warps, half = it >= H;
-            if (live && it < 2 * H && a.out[half]) {
-                const size_t cell = kv8_cell(a.cache, w.page, half, it - half * H, w.off);
-                c[u] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const uint8_t *>(a.cache.codes) + cell * D + base));
-                scale[u] = __ldg(a.cache.scales + cell);
+            const int it = it0 + u * a.row_warps;
+            if (it < 2 * H && a.out[it >= H]) {
+#pragma unroll
+                for (int i = 0; i < kSets; ++i)
+                    if (codes[i]) {
+                        c[u][i] = __ldg(reinterpret_cast<const uint4 *>(codes[i] + size_t(uint32_t(it) * uint32_t(kKv8Page * D))));
+                        scale[u][i] = __ldg(scales[i] + it * kKv8Page);
+                    }
             }
         }
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
             const int it = it0 + u * a.row_warps, half = it >= H;
-            if (live && it < 2 * H && a.out[half]) {
-                T *to = static_cast<T *>(a.out[half]) + row * a.row_stride[half] + (it - half * H) * a.head_stride[half] + base;
-                float x[8];
-                dequantise8(c[u].x, c[u].y, a.cache.format, scale[u], x);
-                store8(to, a.vec[half] != 0, x);
-                dequantise8(c[u].z, c[u].w, a.cache.format, scale[u], x);
-                store8(to + 8, a.vec[half] != 0, x);
+            if (it < 2 * H && a.out[half]) {
+                T *to = static_cast<T *>(a.out[half]) + (it - half * H) * a.head_stride[half] + base;
+#pragma unroll
+                for (int i = 0; i < kSets; ++i)
+                    if (codes[i]) {
+                        T *at = to + row[i] * a.row_stride[half];
+                        float x[8];
+                        dequantise8(c[u][i].x, c[u][i].y, a.cache.format, scale[u][i], x);
+                        store8(at, a.vec[half] != 0, x);
+                        dequantise8(c[u][i].z, c[u][i].w, a.cache.format, scale[u][i], x);
+                        store8(at + 8, a.vec[half] != 0, x);
+                    }
             }
         }
     }
