@@ -263,12 +263,11 @@ struct Unit {
     int head, block, tiles, t0, t1, n_rows, n_pages;
     const int32_t *table;
 };
-// Sequence s's share of it; returns the status of its span.
-__device__ __forceinline__ int fill_unit(const AttnKv8 &p, int s, int tile, Unit &u) {
-    u.rr = kv8_rows(__ldg(p.seqs.row_start + s), __ldg(p.seqs.row_start + s + 1), p.seqs.rows);
-    const int slot = __ldg(p.seqs.slot + s);
+// A sequence's share of it; returns the status of its span.
+__device__ __forceinline__ int fill_unit(const AttnKv8 &p, RowRange rows, int slot, int ctx, int tile, Unit &u) {
+    u.rr = rows;
     int status = 0;
-    u.span = kv8_span(p.cache, slot, __ldg(p.seqs.ctx_len + s), u.rr.r1 - u.rr.r0, &status);
+    u.span = kv8_span(p.cache, slot, ctx, u.rr.r1 - u.rr.r0, &status);
     u.tiles = u.span.total > 0 ? (u.span.total + tile - 1) / tile : 1;
     u.n_rows = (u.rr.r1 - u.rr.r0) * p.group;
     u.table = p.cache.page_table + size_t(u.span.total > 0 ? slot : 0) * p.cache.pages_per_slot;
@@ -296,7 +295,8 @@ __device__ __forceinline__ Unit find_unit(const AttnKv8 &p, const uint32_t *plan
         if (int64_t(plan[mid]) <= w.g) lo = mid; else hi = mid;
     }
     Unit u;
-    fill_unit(p, lo, tile, u);  // its status is reported by plan_tiles
+    fill_unit(p, kv8_rows(__ldg(p.seqs.row_start + lo), __ldg(p.seqs.row_start + lo + 1), p.seqs.rows), __ldg(p.seqs.slot + lo),
+              __ldg(p.seqs.ctx_len + lo), tile, u);  // its status is reported by plan_tiles
     u.head = w.head;
     const uint32_t at = uint32_t(w.g) - plan[lo];
     u.block = int(at / uint32_t(u.tiles));
@@ -314,9 +314,11 @@ __device__ __forceinline__ Unit direct_unit(const AttnKv8 &p, int index, int til
     u.n_rows = 0;
     int before = 0;
     for (int s0 = 0; s0 < p.seqs.n_seqs; s0 += 32) {
-        int blocks = 0;
+        int blocks = 0, slot = -1, ctx = 0;
+        RowRange r{0, 0};
         if (s0 + lane < p.seqs.n_seqs) {
-            const RowRange r = kv8_rows(__ldg(p.seqs.row_start + s0 + lane), __ldg(p.seqs.row_start + s0 + lane + 1), p.seqs.rows);
+            r = kv8_rows(__ldg(p.seqs.row_start + s0 + lane), __ldg(p.seqs.row_start + s0 + lane + 1), p.seqs.rows);
+            slot = __ldg(p.seqs.slot + s0 + lane), ctx = __ldg(p.seqs.ctx_len + s0 + lane);
             blocks = ((r.r1 - r.r0) * p.group + ROWS - 1) / ROWS;
         }
         int sum = blocks;
@@ -328,7 +330,8 @@ __device__ __forceinline__ Unit direct_unit(const AttnKv8 &p, int index, int til
         const uint32_t past = __ballot_sync(0xffffffffu, before + sum > want);
         if (past) {
             const int at = __ffs(past) - 1;
-            *status = fill_unit(p, s0 + at, tile, u);
+            r.r0 = __shfl_sync(0xffffffffu, r.r0, at), r.r1 = __shfl_sync(0xffffffffu, r.r1, at);
+            *status = fill_unit(p, r, __shfl_sync(0xffffffffu, slot, at), __shfl_sync(0xffffffffu, ctx, at), tile, u);
             u.head = index - want * H;
             u.block = want - before - __shfl_sync(0xffffffffu, sum - blocks, at);
             u.t0 = 0, u.t1 = u.tiles;

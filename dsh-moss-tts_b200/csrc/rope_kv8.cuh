@@ -273,26 +273,64 @@ struct RowOp {
     int *status;
 };
 
-// Where row `row` of a batch lies: its sequence s is at or after `first` (searched by the warp, or
-// advanced by a lane).  Returns false where no sequence owns it.
+// The sequence that owns a row: its rows, slot and context.
+struct RowOwner {
+    RowRange r;
+    int slot, ctx;
+};
+// Of rows first .. last (the same in the whole warp), each lane's own `row`.  32 neighbouring sequences
+// around where the rows would lie if all had as many are loaded at once, which finds them in one round
+// trip in batches of up to 32 sequences and of equal ones; a search follows where it does not.
+__device__ __forceinline__ bool row_owner(const mossgpu_seq_batch &q, int first, int last, int row, RowOwner &w) {
+    const int lane = threadIdx.x & 31, n = q.n_seqs;
+    const int b0 = n <= 32 ? 0 : max(0, min(n - 32, int(int64_t(first) * n / q.rows) - 8));
+    const bool in = b0 + lane < n;
+    int start = 0x7fffffff, end = 0x7fffffff, slot = -1, ctx = 0;
+    if (in) {
+        start = __ldg(q.row_start + b0 + lane), end = __ldg(q.row_start + b0 + lane + 1);
+        slot = __ldg(q.slot + b0 + lane), ctx = __ldg(q.ctx_len + b0 + lane);
+    }
+    const bool covered = (b0 == 0 || __shfl_sync(0xffffffffu, start, 0) <= first) && (b0 + 32 >= n || last < __shfl_sync(0xffffffffu, end, 31));
+    int s = -1;  // the last sequence that begins at or before the row
+    if (covered) {
+        if (first == last) {
+            s = __popc(__ballot_sync(0xffffffffu, start <= row)) - 1;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) s += __shfl_sync(0xffffffffu, start, j) <= row;
+        }
+        const int from = max(s, 0);
+        start = __shfl_sync(0xffffffffu, start, from), end = __shfl_sync(0xffffffffu, end, from);
+        slot = __shfl_sync(0xffffffffu, slot, from), ctx = __shfl_sync(0xffffffffu, ctx, from);
+    } else {
+        s = warp_upper_bound(q.row_start, n, first) - 1;
+        while (s + 1 < n && __ldg(q.row_start + s + 1) <= row) ++s;
+        if (s >= 0) {
+            start = __ldg(q.row_start + s), end = __ldg(q.row_start + s + 1);
+            slot = __ldg(q.slot + s), ctx = __ldg(q.ctx_len + s);
+        }
+    }
+    if (s < 0) return false;
+    w.r = kv8_rows(start, end, q.rows);
+    w.slot = slot, w.ctx = ctx;
+    return row >= w.r.r0 && row < w.r.r1;
+}
+
+// Where an owned row lies in the cache; page -1: nowhere (and *status says why).
 struct RowPlace {
     int64_t at;   // position
     int page, off;
 };
-__device__ __forceinline__ bool row_place(const mossgpu_kv8_cache &c, const mossgpu_seq_batch &q, int s, int row, RowPlace &w,
-                                          int *status) {
-    if (s < 0) return false;
-    const RowRange r = kv8_rows(__ldg(q.row_start + s), __ldg(q.row_start + s + 1), q.rows);
-    const int slot = __ldg(q.slot + s), ctx = __ldg(q.ctx_len + s);
-    if (row < r.r0 || row >= r.r1) return false;
-    const SeqSpan span = kv8_span(c, slot, ctx, r.r1 - r.r0, status);
-    w.at = int64_t(ctx) + (row - r.r0);
+__device__ __forceinline__ RowPlace row_place(const mossgpu_kv8_cache &c, const RowOwner &o, int row, int *status) {
+    const SeqSpan span = kv8_span(c, o.slot, o.ctx, o.r.r1 - o.r.r0, status);
+    RowPlace w;
+    w.at = int64_t(o.ctx) + (row - o.r.r0);
     w.page = -1, w.off = 0;
     if (w.at >= 0 && w.at < span.total) {
         w.off = int(w.at % kKv8Page);
-        w.page = kv8_page(c, __ldg(c.page_table + size_t(slot) * c.pages_per_slot + w.at / kKv8Page), status);
+        w.page = kv8_page(c, __ldg(c.page_table + size_t(o.slot) * c.pages_per_slot + w.at / kKv8Page), status);
     }
-    return true;
+    return w;
 }
 
 // q (and, with KV, k) of a row turned, k and v quantised into the cache.  A pass is 32 / LPH heads of one
@@ -313,12 +351,11 @@ __global__ void __launch_bounds__(kRowThreads, 3) k_rope_append(const __grid_con
     if (LAYOUT == kHalves && first < rot) first = in_head * 4, second = first + rot / 2;
     int pos = 0, page = -1, off = 0;
     if (KV) {
-        RowPlace w;
+        RowOwner owner;
+        if (!row_owner(a.seqs, row, row, row, owner)) return;  // the whole warp
         int status = 0;
-        const int s = warp_upper_bound(a.seqs.row_start, a.seqs.n_seqs, row) - 1;
-        const bool owned = row_place(a.cache, a.seqs, s, row, w, &status);
+        const RowPlace w = row_place(a.cache, owner, row, &status);
         if (lane == 0) op_report(a.status, status);
-        if (!owned) return;
         pos = a.pos ? __ldg(a.pos + row) : int(w.at);
         page = w.page, off = w.off;
     } else {
@@ -427,20 +464,19 @@ __global__ void __launch_bounds__(kRowThreads) k_kv8_read(const __grid_constant_
     const int64_t from = int64_t(group) * (kRows * kSets);
     const int part = int(job - group * uint32_t(a.row_warps));
     if (from >= a.seqs.rows) return;
-    const int s0 = warp_upper_bound(a.seqs.row_start, a.seqs.n_seqs, int(from)) - 1;
+    const int row_z = int(min(from + kRows * kSets, int64_t(a.seqs.rows))) - 1;
     const int base = (lane & (kLanes - 1)) * 16, H = a.cache.kv_heads;
     int row[kSets];
     const uint8_t *codes[kSets];  // of the row's position in head 0 of K
     const float *scales[kSets];
 #pragma unroll
     for (int i = 0; i < kSets; ++i) {
-        row[i] = int(min(from + i * kRows + lane / kLanes, int64_t(a.seqs.rows) - 1));  // lanes past the end repeat the last row
-        int s = s0;
-        // further rows may belong to later sequences: the last one that begins at or before the row
-        while (s + 1 < a.seqs.n_seqs && __ldg(a.seqs.row_start + s + 1) <= row[i]) ++s;
-        RowPlace w;
+        row[i] = int(min(from + i * kRows + lane / kLanes, int64_t(row_z)));  // lanes past the end repeat the last row
+        RowOwner owner;
+        const bool owned = row_owner(a.seqs, int(from), row_z, row[i], owner);
+        RowPlace w{};
         int status = 0;
-        const bool owned = row_place(a.cache, a.seqs, s, row[i], w, &status);
+        if (owned) w = row_place(a.cache, owner, row[i], &status);
         op_report(a.status, status);
         codes[i] = nullptr;
         if (owned && w.page >= 0) {
