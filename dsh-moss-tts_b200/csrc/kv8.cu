@@ -15,11 +15,13 @@ size_t type_size(int type) { return type == MOSSGPU_F32 ? 4 : 2; }
 bool is_type(int type) { return type >= MOSSGPU_F32 && type <= MOSSGPU_BF16; }
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
-// 16-byte accesses of 8 elements from every head's multiples of 8
-bool vec_ok(const void *p, int64_t row, int64_t head, int type) {
-    const int64_t e = int64_t(16 / type_size(type));
-    return aligned(p, 16) && row % e == 0 && head % e == 0;
+// Accesses of `bytes` at every head's multiples of them
+bool vec_ok(const void *p, int64_t row, int64_t head, int type, size_t bytes) {
+    const int64_t e = int64_t(bytes / type_size(type));
+    return aligned(p, bytes) && row % e == 0 && head % e == 0;
 }
+// 8 elements
+bool vec8_ok(const void *p, int64_t row, int64_t head, int type) { return vec_ok(p, row, head, type, 8 * type_size(type)); }
 
 int check_cache(const mossgpu_kv8_cache *c, const char *who) {
     if (!c) return op_errorf("%s: cache is NULL", who);
@@ -67,8 +69,8 @@ bool distinct(int rows, int heads, int head_dim, int64_t row, int64_t head) {
 // Warps that share a row (or a few rows) of `passes` passes: one where the rows alone fill the
 // machine, as many as there are passes where they do not.
 int warps_for(int64_t rows, int passes) {
-    const int64_t want = int64_t(kNumSMs) * 32;
-    return int(std::max<int64_t>(1, std::min<int64_t>(passes, (want + rows - 1) / rows)));
+    const int64_t want = int64_t(kNumSMs) * 24;  // resident at once
+    return int(std::max<int64_t>(1, std::min<int64_t>(passes, want / rows)));
 }
 unsigned blocks_for(int64_t warps) { return unsigned((warps + kRowThreads / 32 - 1) / (kRowThreads / 32)); }
 
@@ -230,7 +232,7 @@ int mossgpu_rope_rotate(const mossgpu_rope *rope, const mossgpu_rope_args *args,
     a.out_row_stride = g.out_row_stride, a.out_head_stride = g.out_head_stride;
     a.pos = g.pos;
     a.heads[0] = g.heads;
-    const bool vec = vec_ok(g.x, g.x_row_stride, g.x_head_stride, g.type) && vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
+    const bool vec = vec8_ok(g.x, g.x_row_stride, g.x_head_stride, g.type) && vec8_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
     a.rows = g.rows;
     a.head_dim = g.head_dim;
     a.inverse = g.inverse;
@@ -273,8 +275,8 @@ int mossgpu_kv8_append(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *
     a.pos = g.pos;
     a.heads[0] = g.q ? g.q_heads : 0;
     a.heads[1] = cache->kv_heads;
-    bool vec = !g.q || vec_ok(g.q_out, g.q_out_row_stride, g.q_out_head_stride, g.type);
-    for (int i = g.q ? 0 : 1; i < 3; ++i) vec = vec && vec_ok(a.src[i], a.row_stride[i], a.head_stride[i], g.type);
+    bool vec = !g.q || vec8_ok(g.q_out, g.q_out_row_stride, g.q_out_head_stride, g.type);
+    for (int i = g.q ? 0 : 1; i < 3; ++i) vec = vec && vec8_ok(a.src[i], a.row_stride[i], a.head_stride[i], g.type);
     a.rows = seqs->rows;
     a.head_dim = cache->head_dim;
     a.status = status;
@@ -305,8 +307,8 @@ int mossgpu_kv8_read(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *se
     a.out[0] = g.k, a.out[1] = g.v;
     a.row_stride[0] = g.k_row_stride, a.row_stride[1] = g.v_row_stride;
     a.head_stride[0] = g.k_head_stride, a.head_stride[1] = g.v_head_stride;
-    a.vec[0] = vec_ok(g.k, g.k_row_stride, g.k_head_stride, g.type);
-    a.vec[1] = vec_ok(g.v, g.v_row_stride, g.v_head_stride, g.type);
+    a.vec[0] = vec_ok(g.k, g.k_row_stride, g.k_head_stride, g.type, 32);
+    a.vec[1] = vec_ok(g.v, g.v_row_stride, g.v_head_stride, g.type, 32);
     a.status = status;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);
     const cudaError_t e = g.type == MOSSGPU_F32   ? launch_read<float>(a, st)
@@ -365,8 +367,8 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     p.tile_rows = f.tile_rows;
     p.part_rows = int(std::min<int64_t>(f.tile_rows, int64_t(seqs->rows) * group));
     const int64_t units = (int64_t(seqs->rows) * group / f.tile_rows + seqs->n_seqs) * cache->kv_heads;
-    p.vec_q = vec_ok(g.q, g.q_row_stride, g.q_head_stride, g.type);
-    p.vec_out = vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type);
+    p.vec_q = vec_ok(g.q, g.q_row_stride, g.q_head_stride, g.type, 16);
+    p.vec_out = vec_ok(g.out, g.out_row_stride, g.out_head_stride, g.type, 16);
     p.plan = static_cast<uint32_t *>(g.workspace);
     p.part = reinterpret_cast<float *>(static_cast<char *>(g.workspace) + plan_bytes());
     p.status = status;

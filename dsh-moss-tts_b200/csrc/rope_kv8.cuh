@@ -45,6 +45,19 @@ __device__ __forceinline__ void load8(const T *p, bool vec, float (&x)[8]) {
     for (int i = 0; i < 8; ++i) x[i] = float(p[i]);
 }
 
+// 32 bytes at once: a whole sector of a cache line from one lane.
+__device__ __forceinline__ void load32(const void *p, uint4 &a, uint4 &b) {
+    asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                 : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                 : "l"(p)
+                 : "memory");
+}
+__device__ __forceinline__ void store32(void *p, const uint4 &a, const uint4 &b) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x),
+                 "r"(b.y), "r"(b.z), "r"(b.w)
+                 : "memory");
+}
+
 template <typename T>
 __device__ __forceinline__ void store8(T *p, bool vec, const float (&x)[8]) {
     if (vec) {
@@ -96,7 +109,7 @@ __device__ __forceinline__ float2 rope_angle(int pos, uint64_t step, float magni
 // pairs (2i, 2i + 1) inside the chunks, which lie behind one another: one 16-byte vector in 16-bit types.
 // kHalves: the half layout with a rotary_dim that is a multiple of 8; lane j < rotary_dim / 8 has elements
 // 4j.. and their partners at rotary_dim / 2 + 4j.., the lanes behind it 8 neighbouring ones, so that no
-// element has its partner in another lane.  Both move 8 or 16 bytes at a time.  kAny: either layout, any
+// element has its partner in another lane.  Both move 8 to 32 bytes at a time.  kAny: either layout, any
 // rotary_dim and alignment: element by element, partners by way of shared memory.
 constexpr int kPairs = 0, kHalves = 1, kAny = 2;
 
@@ -113,6 +126,8 @@ __device__ __forceinline__ Raw8<T> raw8(const T *p, int first, int second) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) e[i] = p[first + i], e[4 + i] = p[second + i];
         memcpy(&r, e, sizeof(r));
+    } else if constexpr (sizeof(T) == 4 && LAYOUT == kPairs) {
+        load32(p + first, reinterpret_cast<uint4 *>(&r)[0], reinterpret_cast<uint4 *>(&r)[1]);
     } else if constexpr (sizeof(T) == 4) {
         reinterpret_cast<uint4 *>(&r)[0] = *reinterpret_cast<const uint4 *>(p + first);
         reinterpret_cast<uint4 *>(&r)[1] = *reinterpret_cast<const uint4 *>(p + second);
@@ -134,6 +149,8 @@ __device__ __forceinline__ void put8(T *p, int first, int second, const float (&
     if constexpr (LAYOUT == kAny) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) p[first + i] = e[i], p[second + i] = e[4 + i];
+    } else if constexpr (sizeof(T) == 4 && LAYOUT == kPairs) {
+        store32(p + first, reinterpret_cast<uint4 *>(&r)[0], reinterpret_cast<uint4 *>(&r)[1]);
     } else if constexpr (sizeof(T) == 4) {
         *reinterpret_cast<uint4 *>(p + first) = reinterpret_cast<uint4 *>(&r)[0];
         *reinterpret_cast<uint4 *>(p + second) = reinterpret_cast<uint4 *>(&r)[1];
@@ -223,9 +240,11 @@ __device__ __forceinline__ void rope_turn(float (&x)[8], const LaneRope<LAYOUT> 
     }
 }
 
-// One head of 8-bit codes: the scale from the absolute maximum over the group's lanes (compared
-// as integers, which keeps NaN and infinity above every finite value), codes by an IEEE division
-// and one rounding to nearest even, so that the codes are a function of the values alone.
+// One head of 8-bit codes: the scale from the absolute maximum over the group's lanes (compared as
+// integers, which keeps NaN and infinity above every finite value), codes the nearest to the IEEE quotient
+// x / scale, ties to even: a function of the values alone.  The quotient is first taken by the scale's
+// approximate inverse, within 2^-22 of it; where the quotients 2^-20 below and above round to one code, so
+// does what lies between.  Only a lane that this leaves open (about one in 500) divides.
 template <int LPH>
 __device__ __forceinline__ uint2 quantise8(const float (&x)[8], int format, float *scale_out) {
     uint32_t top = 0;
@@ -240,20 +259,42 @@ __device__ __forceinline__ uint2 quantise8(const float (&x)[8], int format, floa
         scale = __int_as_float(0x7fffffff);
     } else if (scale < 0x1p-126f) {
         scale = 0.f;
-    } else if (format == MOSSGPU_KV_INT8) {
-        uint32_t b[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) b[i] = uint32_t(max(-127, min(127, __float2int_rn(__fdiv_rn(x[i], scale))))) & 0xffu;
-        c.x = b[0] | b[1] << 8 | b[2] << 16 | b[3] << 24;
-        c.y = b[4] | b[5] << 8 | b[6] << 16 | b[7] << 24;
     } else {
-        uint32_t b[4];
+        float inv;
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
+        const float inv_lo = inv * (1.f - 0x1p-20f), inv_hi = inv * (1.f + 0x1p-20f);
+        if (format == MOSSGPU_KV_INT8) {
+            constexpr float kRound = 12582912.f;  // 1.5 * 2^23: the sum's last bits are the nearest whole number
+            uint32_t b[8];
+            bool open = false;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            b[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[2 * i], scale), __fdiv_rn(x[2 * i + 1], scale)),
-                                            __NV_SATFINITE, __NV_E4M3);
-        c.x = b[0] | b[1] << 16;
-        c.y = b[2] | b[3] << 16;
+            for (int i = 0; i < 8; ++i) {
+                b[i] = __float_as_uint(fmaf(x[i], inv_lo, kRound));
+                open |= b[i] != __float_as_uint(fmaf(x[i], inv_hi, kRound));
+            }
+            if (open) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) b[i] = uint32_t(max(-127, min(127, __float2int_rn(__fdiv_rn(x[i], scale)))));
+            }
+            c.x = __byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410);
+            c.y = __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410);
+        } else {
+            uint32_t b[4];
+            bool open = false;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                b[i] = __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv_lo, x[2 * i + 1] * inv_lo), __NV_SATFINITE, __NV_E4M3);
+                open |= b[i] != __nv_cvt_float2_to_fp8x2(make_float2(x[2 * i] * inv_hi, x[2 * i + 1] * inv_hi), __NV_SATFINITE, __NV_E4M3);
+            }
+            if (open) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    b[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(x[2 * i], scale), __fdiv_rn(x[2 * i + 1], scale)), __NV_SATFINITE,
+                                                    __NV_E4M3);
+            }
+            c.x = b[0] | b[1] << 16;
+            c.y = b[2] | b[3] << 16;
+        }
     }
     *scale_out = scale;
     return c;
@@ -336,7 +377,7 @@ __device__ __forceinline__ RowPlace row_place(const mossgpu_kv8_cache &c, const 
 // q (and, with KV, k) of a row turned, k and v quantised into the cache.  A pass is 32 / LPH heads of one
 // tensor; the row's warps take the passes of q, k and v in turn.
 template <typename T, int LPH, int LAYOUT, bool KV>
-__global__ void __launch_bounds__(kRowThreads, 3) k_rope_append(const __grid_constant__ RowOp a) {
+__global__ void __launch_bounds__(kRowThreads, KV ? 4 : 3) k_rope_append(const __grid_constant__ RowOp a) {
     constexpr int kAhead = sizeof(T) == 4 ? 2 : 4;  // passes whose loads are in flight together
     constexpr int kHeads = 32 / LPH;                // heads a pass
     __shared__ __align__(16) float stage[LAYOUT == kAny ? kRowThreads * 8 : 4];
@@ -510,11 +551,21 @@ __global__ void __launch_bounds__(kRowThreads) k_kv8_read(const __grid_constant_
                 for (int i = 0; i < kSets; ++i)
                     if (codes[i]) {
                         T *at = to + row[i] * a.row_stride[half];
-                        float x[8];
-                        dequantise8(c[u][i].x, c[u][i].y, a.cache.format, scale[u][i], x);
-                        store8(at, a.vec[half] != 0, x);
-                        dequantise8(c[u][i].z, c[u][i].w, a.cache.format, scale[u][i], x);
-                        store8(at + 8, a.vec[half] != 0, x);
+                        float x[2][8];
+                        dequantise8(c[u][i].x, c[u][i].y, a.cache.format, scale[u][i], x[0]);
+                        dequantise8(c[u][i].z, c[u][i].w, a.cache.format, scale[u][i], x[1]);
+                        if (a.vec[half]) {
+                            T e[16];
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) e[j] = T(x[j / 8][j % 8]);
+                            uint4 w[sizeof(T)];
+                            memcpy(w, e, sizeof(w));
+#pragma unroll
+                            for (int j = 0; j < int(sizeof(T)); j += 2) store32(reinterpret_cast<char *>(at) + j * 16, w[j], w[j + 1]);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 16; ++j) at[j] = T(x[j / 8][j % 8]);
+                        }
                     }
             }
         }

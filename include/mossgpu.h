@@ -279,7 +279,7 @@ int mossgpu_attention_decode_paged_noalloc(const float *q, const void *kv_layer,
 enum { MOSSGPU_F32 = 0, MOSSGPU_F16 = 1, MOSSGPU_BF16 = 2 };
 
 /* Strides count elements; the innermost dimension is contiguous.  Where the base pointers and
- * strides of a tensor are multiples of 16 bytes it moves 16 bytes at a time, otherwise element
+ * strides of a tensor are multiples of 32 bytes it moves by whole vectors, otherwise element
  * by element. */
 
 /* Rotary positions.  Pair i < rotary_dim / 2 of a head turns by pos * f_i:
