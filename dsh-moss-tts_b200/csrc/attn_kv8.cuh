@@ -32,6 +32,8 @@
 // in fp32.  Statistics, sums and partials are fp32.
 #pragma once
 
+#include <type_traits>
+
 #include "f32x2.cuh"
 #include "rope_kv8.cuh"
 
@@ -770,19 +772,29 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t at) {
 // A thread's share of a tile's codes, to fp16.  Positions that do not exist become zeros.
 template <int D, int FORMAT>
 __device__ __forceinline__ void convert_tile(const uint8_t *raw, uint8_t *to, int left, uint32_t ok) {
-    constexpr int kGran = D / 16;  // 16-byte granules of a row of codes
+    constexpr uint32_t kGran = D / 16, kStep = 128 / kGran;  // 16-byte granules of a row of codes; rows between a thread's granules
+    const uint32_t row = threadIdx.x / kGran, gr = threadIdx.x % kGran;  // row % 8 is the same in all of them
+    raw += threadIdx.x * 16;
+    uint8_t *to_a = to + row * (2 * D) + ((2 * gr) ^ (row & 7)) * 16, *to_b = to + row * (2 * D) + ((2 * gr + 1) ^ (row & 7)) * 16;
+    uint4 w[64 / kStep];
 #pragma unroll
-    for (int i = 0; i < 64 * kGran / 128; ++i) {
-        const int at = int(threadIdx.x) + i * 128, row = at / kGran, gr = at % kGran, pos = row & 31;
-        uint4 w = *reinterpret_cast<const uint4 *>(raw + at * 16);
-        if (pos >= left || !(ok >> (pos >> 4) & 1u)) w = make_uint4(0u, 0u, 0u, 0u);
+    for (int i = 0; i < int(64 / kStep); ++i) w[i] = *reinterpret_cast<const uint4 *>(raw + i * 2048);
+    if (left < kAk8Tile || ok != 3u) {
+#pragma unroll
+        for (int i = 0; i < int(64 / kStep); ++i) {
+            const int pos = int(row + i * kStep) & 31;
+            if (pos >= left || !(ok >> (pos >> 4) & 1u)) w[i] = make_uint4(0u, 0u, 0u, 0u);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < int(64 / kStep); ++i) {
         uint4 a, b;
-        codes_f16<FORMAT>(w.x, a.x, a.y);
-        codes_f16<FORMAT>(w.y, a.z, a.w);
-        codes_f16<FORMAT>(w.z, b.x, b.y);
-        codes_f16<FORMAT>(w.w, b.z, b.w);
-        *reinterpret_cast<uint4 *>(to + row * (2 * D) + ((2 * gr) ^ (row & 7)) * 16) = a;
-        *reinterpret_cast<uint4 *>(to + row * (2 * D) + ((2 * gr + 1) ^ (row & 7)) * 16) = b;
+        codes_f16<FORMAT>(w[i].x, a.x, a.y);
+        codes_f16<FORMAT>(w[i].y, a.z, a.w);
+        codes_f16<FORMAT>(w[i].z, b.x, b.y);
+        codes_f16<FORMAT>(w[i].w, b.z, b.w);
+        *reinterpret_cast<uint4 *>(to_a + i * (kStep * 2 * D)) = a;
+        *reinterpret_cast<uint4 *>(to_b + i * (kStep * 2 * D)) = b;
     }
 }
 
@@ -813,20 +825,17 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                 const int i = 2 * tile + (lane & 1);
                 return tile < t1 && i < u.n_pages ? kv8_page(p.cache, __ldg(u.table + i), &status) : -1;
             };
-            // warp i copies page i & 1's K (i < 2) or V, and its scales
-            const auto issue = [&](int tile, int id) {
+            // warp i copies page i & 1's K (i < 2) or V, and its scales (lanes 0 to 3)
+            const uint8_t *codes = static_cast<const uint8_t *>(p.cache.codes) + ((warp >= 2 ? page_bytes / 2 : 0u) + u.head * kBlock + lane * 16);
+            const float *scales = p.cache.scales + ((warp >= 2 ? H : 0) + u.head) * kKv8Page + (lane & 3) * 4;
+            const uint32_t codes_to = ring_s + warp * kBlock + lane * 16, scales_to = ring_s + 4 * kBlock + warp * 64 + lane * 16;
+            const auto issue = [&](int stage, int id) {
                 const int page = __shfl_sync(0xffffffffu, id, warp & 1);
                 if (page >= 0) {
-                    const uint32_t dst = ring_s + ((tile - t0) % S::kStages) * S::kStage;
-                    const uint8_t *from = static_cast<const uint8_t *>(p.cache.codes) + uint64_t(uint32_t(page)) * page_bytes +
-                                          uint32_t((warp >= 2 ? page_bytes / 2 : 0u) + u.head * kBlock + lane * 16);
+                    const uint8_t *from = codes + uint64_t(uint32_t(page)) * page_bytes;
 #pragma unroll
-                    for (int i = 0; i < kBlock / 512; ++i) cp_async16(dst + warp * kBlock + lane * 16 + i * 512, from + i * 512);
-                    if (lane < 4) {
-                        const float *s = p.cache.scales + uint64_t(uint32_t(page)) * uint32_t(2 * kKv8Page * H) +
-                                         uint32_t(((warp >= 2 ? H : 0) + u.head) * kKv8Page + lane * 4);
-                        cp_async16(dst + 4 * kBlock + warp * 64 + lane * 16, s);
-                    }
+                    for (int i = 0; i < kBlock / 512; ++i) cp_async16(codes_to + stage * S::kStage + i * 512, from + i * 512);
+                    if (lane < 4) cp_async16(scales_to + stage * S::kStage, scales + uint64_t(uint32_t(page)) * uint32_t(2 * kKv8Page * H));
                 }
                 cp_async_commit();
             };
@@ -835,7 +844,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
 #pragma unroll
             for (int i = 0; i < S::kStages; ++i) ids[i] = page_id(t0 + i);
 #pragma unroll
-            for (int i = 0; i < S::kStages - 1; ++i) issue(t0 + i, ids[i]);
+            for (int i = 0; i < S::kStages - 1; ++i) issue(i, ids[i]);
 
             // ---- the query rows as fragments; the sign of the scale goes into them
             const int first = u.block * kRows + warp * kWarpRows;
@@ -879,21 +888,22 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
             cp_async_wait<S::kStages - 2>();
             __syncthreads();
             convert_tile<D, FORMAT>(smem, smem + S::kStage * S::kStages, u.span.total - t0 * kAk8Tile, pages_ok(ids[0]));
-            for (int tile = t0; tile < t1; ++tile) {
+            int stage = 0;
+            for (int tile = t0; tile < t1; ++tile, stage = (stage + 1) % S::kStages) {
                 const uint32_t ok = pages_ok(ids[0]);
                 cp_async_wait<S::kStages - 3>();
                 __syncthreads();  // tile is converted and tile + 1 has arrived for all; tile - 1 is read by none
-                issue(tile + S::kStages - 1, ids[S::kStages - 1]);
+                issue((stage + S::kStages - 1) % S::kStages, ids[S::kStages - 1]);
 #pragma unroll
                 for (int i = 0; i < S::kStages - 1; ++i) ids[i] = ids[i + 1];
                 ids[S::kStages - 1] = page_id(tile + S::kStages);
                 if (tile + 1 < t1)
-                    convert_tile<D, FORMAT>(smem + ((tile + 1 - t0) % S::kStages) * S::kStage,
-                                            smem + S::kStage * S::kStages + ((tile + 1 - t0) & 1) * S::kTile,
+                    convert_tile<D, FORMAT>(smem + ((stage + 1) % S::kStages) * S::kStage,
+                                            smem + S::kStage * S::kStages + ((stage + 1) & 1) * S::kTile,
                                             u.span.total - (tile + 1) * kAk8Tile, pages_ok(ids[0]));
                 if (!any) continue;
-                const float *sc = reinterpret_cast<const float *>(smem + ((tile - t0) % S::kStages) * S::kStage + 4 * kBlock);  // [k, v][32]
-                const uint32_t tile_s = half_s + ((tile - t0) & 1) * S::kTile;
+                const float *sc = reinterpret_cast<const float *>(smem + stage * S::kStage + 4 * kBlock);  // [k, v][32]
+                const uint32_t tile_s = half_s + (stage & 1) * S::kTile;
                 const int p0 = tile * kAk8Tile;
                 const bool whole = p0 + kAk8Tile <= u.span.ctx && ok == 3u;
 
@@ -954,7 +964,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                 }
                 {
                     uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
-                    if (b >= 0x7f800000u || p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
+                    if (b >= 0x7f800000u || (!whole && (p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)))) b = 0;
                     E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
                 }
                 float corr[NR];
@@ -964,8 +974,15 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                                      fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    m[r] = fmaxf(m[r], mx * rf[r]);
-                    const float now = m[r] == -INFINITY ? -INFINITY : m[r] - float(140 - E);
+                    mx *= rf[r];
+                    // kHalf: the reference follows the maximum only when that is 2^6 above it (weights stay below
+                    // 2^14), as the sums have to be multiplied then
+                    if constexpr (MODE == kHalf) {
+                        if (mx > m[r] + 6.f) m[r] = mx;
+                    } else {
+                        m[r] = fmaxf(m[r], mx);
+                    }
+                    const float now = m[r] == -INFINITY ? -INFINITY : m[r] - float((MODE == kHalf ? 134 : 140) - E);
                     const float use = now == -INFINITY ? 0.f : now;
                     corr[r] = ex2(ref[r] - use);
                     ref[r] = now;
@@ -981,25 +998,28 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     l[r] = fmaf(l[r], corr[r], sum.x + sum.y);
                 }
                 uint32_t wa[2][4];  // the weights as the left operand, 16 positions each
+                const auto weights = [&](auto masked) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 v2 = *reinterpret_cast<const float2 *>(sc + 32 + 8 * j + 2 * t);
-                    float2 x[NR];
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 v2 = *reinterpret_cast<const float2 *>(sc + 32 + 8 * j + 2 * t);
+                        float2 x[NR];
 #pragma unroll
-                    for (int r = 0; r < NR; ++r) {
-                        x[r] = mul2(sv[j][r], v2);
-                        if (!whole) {  // a masked position's scale may be anything, NaN included
-                            if (!(seen[r] >> (2 * j) & 1u)) x[r].x = 0.f;
-                            if (!(seen[r] >> (2 * j + 1) & 1u)) x[r].y = 0.f;
+                        for (int r = 0; r < NR; ++r) {
+                            x[r] = mul2(sv[j][r], v2);
+                            if constexpr (decltype(masked)::value) {  // a masked position's scale may be anything, NaN included
+                                if (!(seen[r] >> (2 * j) & 1u)) x[r].x = 0.f;
+                                if (!(seen[r] >> (2 * j + 1) & 1u)) x[r].y = 0.f;
+                            }
+                        }
+                        if constexpr (MODE == kSplit) {
+                            wa[j / 2][2 * (j & 1)] = split2(x[0], &wa[j / 2][2 * (j & 1) + 1]);
+                        } else {
+                            wa[j / 2][2 * (j & 1)] = pack2(x[0]);
+                            wa[j / 2][2 * (j & 1) + 1] = pack2(x[NR - 1]);
                         }
                     }
-                    if constexpr (MODE == kSplit) {
-                        wa[j / 2][2 * (j & 1)] = split2(x[0], &wa[j / 2][2 * (j & 1) + 1]);
-                    } else {
-                        wa[j / 2][2 * (j & 1)] = pack2(x[0]);
-                        wa[j / 2][2 * (j & 1) + 1] = pack2(x[NR - 1]);
-                    }
-                }
+                };
+                if (whole) weights(std::false_type()); else weights(std::true_type());
                 if constexpr (MODE == kHalf) {
                     // the sums stay in the products' accumulators; most tiles raise no maximum
                     if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[NR - 1] != 1.f)) {
