@@ -1,9 +1,9 @@
 // logprob.cu -- log-probabilities of given tokens, entropy and the most likely tokens of rows of
 // logits (mossgpu_token_logprobs).
 //
-// A row is held in registers, 2 or 8 vectors of 16 bytes a thread, by one CTA or by a cluster of
-// up to 16: it is read from HBM once, and the maximum, the sums and the selection all work on what
-// was read.  With x the logits, M = max x, t = (x - M) log2(e) / T:
+// A row is held by one CTA or by a cluster of up to 16, 2 or 8 vectors of 16 bytes a thread in
+// registers or 8 in registers and 8 in shared memory: it is read from HBM once, and the maximum, the
+// sums and the selection all work on what was read.  With x the logits, M = max x, t = (x - M) log2(e) / T:
 //   Z = sum 2^t,  S = sum 2^t t,
 //   log p_i = (x_i - M) / T - ln Z,  entropy = ln Z - ln 2 S / Z.
 // CTAs of a cluster sum against their own maxima; rank 0 merges.
@@ -137,9 +137,10 @@ __device__ __noinline__ int select_exact(const T *x_row, int vocab, int top_k, i
     return *sum;
 }
 
-// NT threads hold NV vectors each; `ctas` CTAs a row.
+// NT threads hold NV vectors each, those from the eighth on in their own places in shared memory (twice
+// as many rows are in flight then as registers alone hold); `ctas` CTAs a row.
 template <typename T, int NT, int NV>
-__global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT) k_token_logprobs(
+__global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprobs(
     const __grid_constant__ mossgpu_logprob_args a, int ctas, int *status) {
     constexpr int VE = 16 / int(sizeof(T));
     // candidates a CTA ranks; 32 groups of a uniform row give about 130 at k = 32
@@ -157,23 +158,41 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT
     if (tid == 0) n_cand = 0;
 
     // ---- the row; vector v holds elements v VE - lead ..
-    uint4 x[NV];
+    constexpr int NR = NV < 8 ? NV : 8;
+    extern __shared__ __align__(16) uint4 parked[];  // [NV - 8][NT]
+    uint4 x[NR];
+    const auto vec = [&](int v) { return v < NR ? x[v] : parked[(v - NR) * NT + tid]; };
     const auto id_of = [=](int v, int i) { return ((v * ctas + rank) * NT + tid) * VE - lead + i; };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int e0 = id_of(v, 0);
-        if (e0 >= 0 && e0 + VE <= a.vocab) {
-            x[v] = __ldg(reinterpret_cast<const uint4 *>(x_row + e0));
-        } else {
+        const bool in = e0 >= 0 && e0 + VE <= a.vocab;
+        uint4 edge;
+        if (!in) {
             T e[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) e[i] = e0 + i >= 0 && e0 + i < a.vocab ? x_row[e0 + i] : T(-INFINITY);
-            memcpy(&x[v], e, 16);
+            memcpy(&edge, e, 16);
+        }
+        if (v < NR) {
+            x[v] = edge;
+            if (in) x[v] = __ldg(reinterpret_cast<const uint4 *>(x_row + e0));
+        } else {
+            uint4 *to = parked + (v - NR) * NT + tid;
+            if (in)
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(x_row + e0) : "memory");
+            else
+                *to = edge;
         }
     }
     float mine = largest<T>(x[0]);
 #pragma unroll
-    for (int v = 1; v < NV; ++v) mine = max_nan(mine, largest<T>(x[v]));
+    for (int v = 1; v < NR; ++v) mine = max_nan(mine, largest<T>(x[v]));
+    if constexpr (NV > NR) {
+        asm volatile("cp.async.wait_all;" ::: "memory");  // a thread reads its own places alone
+#pragma unroll
+        for (int v = NR; v < NV; ++v) mine = max_nan(mine, largest<T>(vec(v)));
+    }
     float group = mine;
 #pragma unroll
     for (int o = 1; o < NT / 32; o <<= 1) group = max_nan(group, __shfl_xor_sync(0xffffffffu, group, o));
@@ -207,14 +226,16 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT
 #pragma unroll
             for (int w = 0; w < kWords; ++w) in[w] = 0;
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
+            for (int v = 0; v < NV; ++v) {
+                const uint4 y = vec(v);
 #pragma unroll
                 for (int i = 0; i < VE / 2; ++i) {
-                    const float2 f = pair_of<T>(x[v], i);
+                    const float2 f = pair_of<T>(y, i);
                     const int bit = (v * VE + 2 * i) % 32;
                     if (f.x >= least) in[(v * VE) / 32] |= 1u << bit;
                     if (f.y >= least) in[(v * VE) / 32] |= 2u << bit;
                 }
+            }
             if (few) {
 #pragma unroll
                 for (int v = 0; v < NV; ++v) {
@@ -243,15 +264,17 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT
     if (fabsf(off) < 1e30f) {
         miss = fmaf(top, c, off);
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
+        for (int v = 0; v < NV; ++v) {
+            const uint4 y = vec(v);
 #pragma unroll
             for (int i = 0; i < VE / 2; ++i) {
-                const float2 f = pair_of<T>(x[v], i);
+                const float2 f = pair_of<T>(y, i);
                 const float t0 = fmaxf(fmaf(f.x, c, off), -200.f), t1 = fmaxf(fmaf(f.y, c, off), -200.f);
                 const float e0 = ex2(t0), e1 = ex2(t1);  // 2^-200 is 0, and 0 * infinity stays out of the sum
                 z += e0, s = fmaf(e0, t0, s);
                 z += e1, s = fmaf(e1, t1, s);
             }
+        }
     } else {
 #pragma unroll 1
         for (int v = 0; v < NV * VE; ++v) {
@@ -370,6 +393,11 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : NT == 1024 ? 1 : 1024 / NT
 template <typename T, int NT, int NV>
 cudaError_t launch(const mossgpu_logprob_args &a, int ctas, int *status, cudaStream_t st) {
     auto *kernel = k_token_logprobs<T, NT, NV>;
+    const int smem = NV > 8 ? (NV - 8) * NT * 16 : 0;
+    if (smem > 0) {
+        const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+    }
     if (ctas > 8) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
         if (e != cudaSuccess) return e;
@@ -377,6 +405,7 @@ cudaError_t launch(const mossgpu_logprob_args &a, int ctas, int *status, cudaStr
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(unsigned(a.rows) * unsigned(ctas));
     cfg.blockDim = dim3(NT);
+    cfg.dynamicSmemBytes = size_t(smem);
     cfg.stream = st;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
@@ -402,10 +431,10 @@ cudaError_t dispatch(const mossgpu_logprob_args &a, int *status, cudaStream_t st
     }
     if (n <= 8 * 32) return launch<T, 32, 8>(a, 1, status, st);
     if (n <= 8 * 128) return launch<T, 128, 8>(a, 1, status, st);
+    if (n <= 8 * 512) return launch<T, 512, 8>(a, 1, status, st);
     int ctas = 1;
-    while (ctas < kLpMaxCluster && n > 8 * 512 * ctas) ctas *= 2;
-    if (n <= 8 * 512 * ctas) return launch<T, 512, 8>(a, ctas, status, st);
-    return launch<T, 1024, 8>(a, ctas, status, st);
+    while (ctas < kLpMaxCluster && n > 16 * 512 * ctas) ctas *= 2;
+    return launch<T, 512, 16>(a, ctas, status, st);
 }
 
 }  // namespace
