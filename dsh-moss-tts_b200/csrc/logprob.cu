@@ -139,9 +139,10 @@ __device__ __noinline__ int select_exact(const T *x_row, int vocab, int top_k, i
 
 // NT threads hold NV vectors each, those from the eighth on in their own places in shared memory (twice
 // as many rows are in flight then as registers alone hold); `ctas` CTAs a row.
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool CLUSTER>
 __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprobs(
-    const __grid_constant__ mossgpu_logprob_args a, int ctas, int *status) {
+    const __grid_constant__ mossgpu_logprob_args a, int cluster_ctas, int *status) {
+    const int ctas = CLUSTER ? cluster_ctas : 1;
     constexpr int VE = 16 / int(sizeof(T));
     // candidates a CTA ranks; 32 groups of a uniform row give about 130 at k = 32
     constexpr int kCandidates = NT == 32 ? 256 : 512;
@@ -149,25 +150,25 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
     __shared__ float2 warp_sums[NT / 32];
     __shared__ unsigned long long cand[kCandidates];
     __shared__ int n_cand;
-    __shared__ LpPart parts[NT < 512 ? 1 : kLpMaxCluster];  // clusters have CTAs of 512 threads or more
+    __shared__ LpPart parts[CLUSTER ? kLpMaxCluster : 1];
     const int tid = threadIdx.x, lane = tid & 31;
-    const int row = blockIdx.x / ctas, rank = blockIdx.x - row * ctas;
+    const int row = CLUSTER ? blockIdx.x / ctas : blockIdx.x, rank = CLUSTER ? blockIdx.x - row * ctas : 0;
     const T *x_row = static_cast<const T *>(a.logits) + int64_t(row) * a.row_stride;
     const int lead = int((reinterpret_cast<uintptr_t>(x_row) / sizeof(T)) % VE);  // elements past a 16-byte boundary
-    if (ctas > 1) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
+    if constexpr (CLUSTER) asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
     if (tid == 0) n_cand = 0;
 
     // ---- the row; vector v holds elements v VE - lead ..
     constexpr int NR = NV < 8 ? NV : 8;
     extern __shared__ __align__(16) uint4 parked[];  // [NV - 8][NT]
     uint4 x[NR];
-    const auto vec = [&](int v) { return v < NR ? x[v] : parked[(v - NR) * NT + tid]; };
+    const auto vec = [&](int v) -> uint4 { return v < NR ? x[v] : parked[(v - NR) * NT + tid]; };
     const auto id_of = [=](int v, int i) { return ((v * ctas + rank) * NT + tid) * VE - lead + i; };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int e0 = id_of(v, 0);
         const bool in = e0 >= 0 && e0 + VE <= a.vocab;
-        uint4 edge;
+        uint4 edge = make_uint4(0u, 0u, 0u, 0u);
         if (!in) {
             T e[VE];
 #pragma unroll
@@ -296,7 +297,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
 
     // ---- the CTA's share
     LpPart *mine_part = &parts[rank];
-    if (ctas > 1) {
+    if constexpr (CLUSTER) {
         asm volatile("barrier.cluster.wait.aligned;" ::: "memory");  // rank 0 runs, its shared memory may be written
         mine_part = cg::this_cluster().map_shared_rank(&parts[rank], 0);
     }
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
             mine_part->count = min(n, a.top_k);
         }
     }
-    if (ctas > 1) {
+    if constexpr (CLUSTER) {
         asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
         if (rank != 0) return;
     } else {
@@ -328,7 +329,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
 
     // ---- rank 0: the row
     float m = parts[0].top, zz = parts[0].z, ss = parts[0].s;
-    if (ctas > 1) {
+    if constexpr (CLUSTER) {
         for (int r = 1; r < ctas; ++r) m = max_nan(m, parts[r].top);
         zz = ss = 0.f;
         for (int r = 0; r < ctas; ++r) {
@@ -358,41 +359,52 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
         if (a.entropy) a.entropy[row] = bad ? nan : empty ? 0.f : (log_z - ss / zz) * kLpLn2;
     }
     if (a.top_k == 0) return;
-    if (ctas == 1) {
+    if constexpr (!CLUSTER) {
         for (int i = tid; i < a.top_k; i += NT) {  // a CTA has the whole row: top_k <= vocab entries are there
             const unsigned long long key = parts[0].best[i];
             const int64_t to = int64_t(row) * a.top_k + i;
             if (a.top_ids) a.top_ids[to] = int32_t(~uint32_t(key));
             if (a.top_logprobs) a.top_logprobs[to] = logprob(order_value(uint32_t(key >> 32)));
         }
-        return;
-    }
-    // merge the parts' sorted lists: an entry's rank is its own plus, of every other part, how many are larger
-    for (int i = tid; i < ctas * kLpMaxTop; i += NT) {
-        const int r = i / kLpMaxTop, j = i % kLpMaxTop;
-        if (j >= parts[r].count) continue;
-        const unsigned long long key = parts[r].best[j];
-        int at = j;
-        for (int q = 0; q < ctas; ++q) {
-            if (q == r) continue;
+    } else {
+        // merge the parts' sorted lists: an entry's place is its own plus, of every other part, how many are
+        // larger.  The largest of the parts' k-th entries bounds the k-th from below, which leaves few.
+        __shared__ int place[kLpMaxCluster * kLpMaxTop];
+        unsigned long long least = lane < ctas && parts[lane].count >= a.top_k ? parts[lane].best[a.top_k - 1] : 0ull;
+#pragma unroll
+        for (int o = kLpMaxCluster / 2; o > 0; o >>= 1) least = max(least, __shfl_xor_sync(0xffffffffu, least, o));
+        least = __shfl_sync(0xffffffffu, least, 0);
+        const int entries = ctas * a.top_k;
+        for (int i = tid; i < entries; i += NT) place[i] = i % a.top_k;
+        __syncthreads();
+        for (int i = tid; i < entries * ctas; i += NT) {
+            const int e = i / ctas, q = i - e * ctas, r = e / a.top_k, j = e - r * a.top_k;
+            if (q == r || j >= parts[r].count) continue;
+            const unsigned long long key = parts[r].best[j];
+            if (key < least) continue;
             int lo = 0, hi = parts[q].count;
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
                 if (parts[q].best[mid] > key) lo = mid + 1; else hi = mid;
             }
-            at += lo;
+            if (lo > 0) atomicAdd(place + e, lo);
         }
-        if (at < a.top_k) {
-            const int64_t to = int64_t(row) * a.top_k + at;
+        __syncthreads();
+        for (int e = tid; e < entries; e += NT) {
+            const int r = e / a.top_k, j = e - r * a.top_k;
+            if (j >= parts[r].count) continue;
+            const unsigned long long key = parts[r].best[j];
+            if (key < least || place[e] >= a.top_k) continue;
+            const int64_t to = int64_t(row) * a.top_k + place[e];
             if (a.top_ids) a.top_ids[to] = int32_t(~uint32_t(key));
             if (a.top_logprobs) a.top_logprobs[to] = logprob(order_value(uint32_t(key >> 32)));
         }
     }
 }
 
-template <typename T, int NT, int NV>
+template <typename T, int NT, int NV, bool CLUSTER = false>
 cudaError_t launch(const mossgpu_logprob_args &a, int ctas, int *status, cudaStream_t st) {
-    auto *kernel = k_token_logprobs<T, NT, NV>;
+    auto *kernel = k_token_logprobs<T, NT, NV, CLUSTER>;
     const int smem = NV > 8 ? (NV - 8) * NT * 16 : 0;
     if (smem > 0) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -412,7 +424,7 @@ cudaError_t launch(const mossgpu_logprob_args &a, int ctas, int *status, cudaStr
     at[0].val.clusterDim.x = unsigned(ctas);
     at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = ctas > 1 ? 1 : 0;
+    cfg.numAttrs = CLUSTER ? 1 : 0;
     return cudaLaunchKernelEx(&cfg, kernel, a, ctas, status);
 }
 
@@ -422,19 +434,24 @@ cudaError_t dispatch(const mossgpu_logprob_args &a, int *status, cudaStream_t st
     constexpr int VE = 16 / int(sizeof(T));
     const bool even = reinterpret_cast<uintptr_t>(a.logits) % 16 == 0 && (a.row_stride % VE == 0 || a.rows == 1);
     const int n = (a.vocab + (even ? 0 : VE - 1) + VE - 1) / VE;
-    // Two vectors a thread where all rows' threads are resident at once: a row's latency is what its
-    // longest thread does.  Eight otherwise: the per-row work is spread over more logits.
-    if (int64_t(a.rows) * n <= int64_t(2) * 148 * 1024) {
+    // Two or four vectors a thread where all rows' threads are resident at once: a row's latency is what its
+    // longest thread does (one row of 128001 logits: 10.8 us against 14.8 with 16 vectors, 12.9 on 16 CTAs).
+    // More otherwise: the per-row work is spread over more logits (160 such rows: 30 us against 41 with four).
+    const int64_t threads = int64_t(148) * 1024;
+    if (int64_t(a.rows) * n <= 2 * threads) {
         if (n <= 2 * 128) return launch<T, 128, 2>(a, 1, status, st);
-        for (int ctas = 1; ctas <= kLpMaxCluster; ctas *= 2)
-            if (n <= 2 * 512 * ctas) return launch<T, 512, 2>(a, ctas, status, st);
+        if (n <= 2 * 512) return launch<T, 512, 2>(a, 1, status, st);
+        for (int ctas = 2; ctas <= 8; ctas *= 2)
+            if (n <= 2 * 512 * ctas) return launch<T, 512, 2, true>(a, ctas, status, st);
+        if (n <= 4 * 512 * 8) return launch<T, 512, 4, true>(a, 8, status, st);
     }
     if (n <= 8 * 32) return launch<T, 32, 8>(a, 1, status, st);
     if (n <= 8 * 128) return launch<T, 128, 8>(a, 1, status, st);
     if (n <= 8 * 512) return launch<T, 512, 8>(a, 1, status, st);
-    int ctas = 1;
+    if (n <= 16 * 512) return launch<T, 512, 16>(a, 1, status, st);
+    int ctas = 2;
     while (ctas < kLpMaxCluster && n > 16 * 512 * ctas) ctas *= 2;
-    return launch<T, 512, 16>(a, ctas, status, st);
+    return launch<T, 512, 16, true>(a, ctas, status, st);
 }
 
 }  // namespace
