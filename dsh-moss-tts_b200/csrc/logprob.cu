@@ -161,30 +161,28 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
     // ---- the row; vector v holds elements v VE - lead ..
     constexpr int NR = NV < 8 ? NV : 8;
     extern __shared__ __align__(16) uint4 parked[];  // [NV - 8][NT]
-    uint4 x[NR];
+    uint4 x[NR] = {};
     const auto vec = [&](int v) -> uint4 { return v < NR ? x[v] : parked[(v - NR) * NT + tid]; };
     const auto id_of = [=](int v, int i) { return ((v * ctas + rank) * NT + tid) * VE - lead + i; };
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
         const int e0 = id_of(v, 0);
-        const bool in = e0 >= 0 && e0 + VE <= a.vocab;
-        uint4 edge = make_uint4(0u, 0u, 0u, 0u);
-        if (!in) {
+        uint4 y;
+        if (e0 >= 0 && e0 + VE <= a.vocab) {
+            if (v >= NR) {
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(parked + (v - NR) * NT + tid))),
+                             "l"(x_row + e0)
+                             : "memory");
+                continue;
+            }
+            y = __ldg(reinterpret_cast<const uint4 *>(x_row + e0));
+        } else {
             T e[VE];
 #pragma unroll
             for (int i = 0; i < VE; ++i) e[i] = e0 + i >= 0 && e0 + i < a.vocab ? x_row[e0 + i] : T(-INFINITY);
-            memcpy(&edge, e, 16);
+            memcpy(&y, e, 16);
         }
-        if (v < NR) {
-            x[v] = edge;
-            if (in) x[v] = __ldg(reinterpret_cast<const uint4 *>(x_row + e0));
-        } else {
-            uint4 *to = parked + (v - NR) * NT + tid;
-            if (in)
-                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(uint32_t(__cvta_generic_to_shared(to))), "l"(x_row + e0) : "memory");
-            else
-                *to = edge;
-        }
+        if (v < NR) x[v] = y; else parked[(v - NR) * NT + tid] = y;
     }
     float mine = largest<T>(x[0]);
 #pragma unroll
