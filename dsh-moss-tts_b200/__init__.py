@@ -56,6 +56,7 @@ EXPORTS = [
     "mossgpu_codec_profile", "mossgpu_codec_profile_read", "mossgpu_codec_kernel_name", "mossgpu_codec_status",
     "mossgpu_rope_steps", "mossgpu_rope_rotate", "mossgpu_kv8_append", "mossgpu_kv8_read",
     "mossgpu_attention_kv8_workspace_bytes", "mossgpu_attention_kv8", "mossgpu_token_logprobs",
+    "mossgpu_frame_logprobs",
 ]
 
 
@@ -246,6 +247,8 @@ def lib() -> C.CDLL:
         L.mossgpu_attention_kv8_workspace_bytes.argtypes = [C.POINTER(KV8Cache), C.c_int, C.c_int]
         L.mossgpu_attention_kv8.argtypes = [C.POINTER(KV8Cache), C.POINTER(SeqBatch), C.POINTER(AttentionKV8Args),
                                             C.c_void_p]
+        L.mossgpu_frame_logprobs.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_float, C.c_void_p, C.c_void_p,
+                                             C.c_void_p, C.c_void_p]
         L.mossgpu_token_logprobs.argtypes = [C.POINTER(LogprobArgs), C.c_void_p]
         _LIB = L
         return L
@@ -370,6 +373,17 @@ class Engine:
         self._check(self.lib.mossgpu_step(self.h, sids, n, C.byref(params), _ptr(f), codes, _ptr(stop), _ptr(logits),
                                           _ptr(gate), int(run_global)))
         return codes, stop.astype(bool), gate, logits
+
+    def frame_logprobs(self, n: int, codes=None, top_k: int = 0, temperature: float = 1.0):
+        """Under the audio logits of the last step call (its n streams): (logprob[n][16] of `codes`, or of that
+        step's own codes, entropy[n][16], top_ids[n][16][top_k], top_logprobs[n][16][top_k])."""
+        c = None if codes is None else np.ascontiguousarray(codes, np.int32).reshape(n, NVQ)
+        lp, ent = np.zeros((n, NVQ), np.float32), np.zeros((n, NVQ), np.float32)
+        ids = np.zeros((n, NVQ, top_k), np.int32) if top_k > 0 else None
+        top = np.zeros((n, NVQ, top_k), np.float32) if top_k > 0 else None
+        self._check(self.lib.mossgpu_frame_logprobs(self.h, _ptr(c), n, top_k, temperature, _ptr(lp), _ptr(ent), _ptr(ids),
+                                                    _ptr(top)))
+        return lp, ent, ids, top
 
     def step_frames(self, sids, params: SampleParams, n_frames: int, want_codes=True):
         """n_frames free-running frames on the device.  Returns (codes[n_frames][n][16], frames_done[n])."""

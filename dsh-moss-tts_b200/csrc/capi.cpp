@@ -168,6 +168,13 @@ int mossgpu_step(mossgpu_engine *e, const int32_t *stream_ids, int n, const moss
     });
 }
 
+int mossgpu_frame_logprobs(mossgpu_engine *e, const int32_t *codes, int n, int top_k, float temperature, float *logprob,
+                           float *entropy, int32_t *top_ids, float *top_logprobs) {
+    return guarded(e, [&](mossgpu::Engine &g) {
+        g.frame_logprobs(codes, n, top_k, temperature, logprob, entropy, top_ids, top_logprobs);
+    });
+}
+
 int mossgpu_step_frames(mossgpu_engine *e, const int32_t *stream_ids, int n, const mossgpu_sample_params *params,
                         int n_frames, int32_t *out_codes, int32_t *out_frames_done) {
     return guarded(e, [&](mossgpu::Engine &g) {

@@ -1,6 +1,7 @@
 // engine.cu -- host side of the B200 engine: .moss upload + repack, the paged KV cache,
 // stream slots, and the launch sequences of one frame (local decoder, gate, codes, global
 // step) and of a prefill.  Exposed through the C ABI in capi.cpp (include/mossgpu.h).
+#include "../../include/mossgpu.h"
 #include "engine.h"
 
 #include <cuda_runtime.h>
@@ -1384,6 +1385,7 @@ void Engine::step(const int32_t *sids, int n, const SampleParamsC &p, const int3
     if (n <= 0) return;
     if (n > max_streams_) throw std::runtime_error("batch larger than max_streams");
     launches_ = 0;
+    logit_rows_ = 0;
     std::vector<int> upd;
     std::vector<char> seen(size_t(max_streams_), 0);
     for (int r = 0; r < n; ++r) {
@@ -1456,6 +1458,42 @@ void Engine::step(const int32_t *sids, int n, const SampleParamsC &p, const int3
         }
     }
     if (out_logits) std::memcpy(out_logits, h_logits, size_t(R) * kNVq * kCodebook * sizeof(float));
+    logit_rows_ = R;
+}
+
+void Engine::frame_logprobs(const int32_t *codes, int n, int top_k, float temperature, float *logprob, float *entropy,
+                            int32_t *top_ids, float *top_logprobs) {
+    if (n <= 0 || n != logit_rows_) throw std::runtime_error("frame_logprobs: n is not the number of streams of the last step call");
+    if (codes && !logprob) throw std::runtime_error("frame_logprobs: codes without logprob");
+    const size_t rows = size_t(n) * kNVq, most = size_t(max_streams_) * kNVq;
+    if (codes)
+        for (size_t i = 0; i < rows; ++i)
+            if (codes[i] >= kCodebook) throw std::runtime_error("frame_logprobs: code out of range");
+    if (top_k < 0 || top_k > 32) throw std::runtime_error("frame_logprobs: top_k must be 0 .. 32");
+    if (!lp_buf_) lp_buf_ = dalloc<float>(most * (3 + 2 * 32), owned_);
+    int32_t *d_codes = static_cast<int32_t *>(lp_buf_);
+    float *d_lp = reinterpret_cast<float *>(d_codes + most), *d_ent = d_lp + most, *d_top = d_ent + most;
+    int32_t *d_ids = reinterpret_cast<int32_t *>(d_top + most * 32);
+    if (codes) CK(cudaMemcpyAsync(d_codes, codes, rows * sizeof(int32_t), cudaMemcpyHostToDevice, stream_));
+    mossgpu_logprob_args a{};
+    a.logits = logits_;
+    a.tokens = logprob ? (codes ? d_codes : codes_) : nullptr;  // without codes: the step's own predictions
+    a.logprob = logprob ? d_lp : nullptr;
+    a.entropy = entropy ? d_ent : nullptr;
+    a.top_ids = top_ids ? d_ids : nullptr;
+    a.top_logprobs = top_logprobs ? d_top : nullptr;
+    a.row_stride = kCodebook;
+    a.rows = int(rows);
+    a.vocab = kCodebook;
+    a.type = MOSSGPU_F32;
+    a.top_k = top_k;
+    a.temperature = temperature;
+    if (mossgpu_token_logprobs(&a, stream_) != 0) throw std::runtime_error(mossgpu_op_last_error());
+    if (logprob) CK(cudaMemcpyAsync(logprob, d_lp, rows * sizeof(float), cudaMemcpyDeviceToHost, stream_));
+    if (entropy) CK(cudaMemcpyAsync(entropy, d_ent, rows * sizeof(float), cudaMemcpyDeviceToHost, stream_));
+    if (top_ids) CK(cudaMemcpyAsync(top_ids, d_ids, rows * top_k * sizeof(int32_t), cudaMemcpyDeviceToHost, stream_));
+    if (top_logprobs) CK(cudaMemcpyAsync(top_logprobs, d_top, rows * top_k * sizeof(float), cudaMemcpyDeviceToHost, stream_));
+    CK(cudaStreamSynchronize(stream_));
 }
 
 // n_frames consecutive frames for n streams without a host round trip between frames: the
@@ -1466,6 +1504,7 @@ void Engine::step(const int32_t *sids, int n, const SampleParamsC &p, const int3
 void Engine::step_frames(const int32_t *sids, int n, const SampleParamsC &p, int n_frames, int32_t *out_codes,
                          int32_t *out_frames_done) {
     if (n <= 0 || n_frames <= 0) return;
+    logit_rows_ = 0;  // of no one frame afterwards
     if (n > max_streams_) throw std::runtime_error("batch larger than max_streams");
     if (n_frames > kMaxFramesPerCall) throw std::runtime_error("n_frames above the per-call limit");
     std::vector<int> upd;

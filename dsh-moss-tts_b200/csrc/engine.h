@@ -89,6 +89,9 @@ public:
     void step(const int32_t *sids, int n, const SampleParamsC &p, const int32_t *forced, int32_t *out_codes,
               uint8_t *out_stop, float *out_logits, float *out_gate, bool run_global);
     static constexpr int kMaxFramesPerCall = 1024;
+    // Log-probabilities under the audio logits of the last step() (n rows of it), see mossgpu_frame_logprobs.
+    void frame_logprobs(const int32_t *codes, int n, int top_k, float temperature, float *logprob, float *entropy,
+                        int32_t *top_ids, float *top_logprobs);
     void step_frames(const int32_t *sids, int n, const SampleParamsC &p, int n_frames, int32_t *out_codes,
                      int32_t *out_frames_done);
     void global_step_embed(const int32_t *sids, int n, const float *x, float *hidden_out);
@@ -219,6 +222,8 @@ private:
     float2 *rope_ = nullptr;
     // row-batch scratch
     float *x_ = nullptr, *lx_ = nullptr, *q_ = nullptr, *attn_ = nullptr, *mlp_ = nullptr, *logits_ = nullptr;
+    int logit_rows_ = 0;           // rows of logits_ that the last step() left; 0: none
+    void *lp_buf_ = nullptr;       // frame_logprobs: tokens, log-probabilities, entropies, ids, their log-probabilities
     int *plan_ = nullptr, *work_ = nullptr, *active_ = nullptr, *codes_ = nullptr, *used_ = nullptr;
     float *part_ = nullptr, *gate_ = nullptr;
     int4 *desc_ = nullptr;  // decode-attention chunk descriptors

@@ -352,6 +352,7 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     const AttnForm f = attn_form(*cache, g.type, seqs->rows, seqs->n_seqs, group);
     const int64_t jobs = int64_t(seqs->rows) * g.q_heads;
     if (jobs > (int64_t(1) << 33)) return op_errorf("%s: rows * q_heads is above 2^33", who);
+    if (int64_t(seqs->rows) * (g.q_heads / cache->kv_heads) > (1 << 30)) return op_errorf("%s: rows times heads of a group are above 2^30", who);
     // the plan counts tiles in 32 bits
     const int64_t blocks = int64_t(seqs->rows) * group / f.tile_rows + seqs->n_seqs;
     if (blocks * (cache->pages_per_slot / 2 + 1) > INT64_C(0x7fffffff))

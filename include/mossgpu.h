@@ -119,6 +119,19 @@ int mossgpu_step(mossgpu_engine *e, const int32_t *stream_ids, int n, const moss
                  const int32_t *forced, int32_t *out_codes, uint8_t *out_stop, float *out_logits, float *out_gate,
                  int run_global);
 
+/* Log-probabilities under the audio logits that the last mossgpu_step call of this engine left on the
+ * device (its n streams in its order; mossgpu_step_frames leaves none): softmax(logits / temperature) of
+ * each of the 16 channels, before the repetition penalty.
+ *   codes        [n][16] the codes to score, a negative one for none (0); NULL = the call's out_codes
+ *   logprob      [n][16], or NULL
+ *   entropy      [n][16] in nats, or NULL
+ *   top_ids      [n][16][top_k] the most likely codes (equal logits: the lower code first), or NULL
+ *   top_logprobs [n][16][top_k], or NULL; top_k 0 .. 32, 0 without both
+ * Values of a stream whose gate ended it in that call are void.  Scores forced or drafted codes without
+ * bringing the logits to the host (mossgpu_token_logprobs is the operator). */
+int mossgpu_frame_logprobs(mossgpu_engine *e, const int32_t *codes, int n, int top_k, float temperature, float *logprob,
+                           float *entropy, int32_t *top_ids, float *top_logprobs);
+
 /* n_frames consecutive frames of generate() for n streams in one call, free-running (no
  * teacher forcing), with no host round trip between frames: positions, frame indices and
  * the end gate advance on the device.  out_codes [n_frames][n][16] holds -1 for frames after
@@ -268,8 +281,9 @@ int mossgpu_attention_decode_paged_noalloc(const float *q, const void *kv_layer,
  * Standalone ops in the manner of mossgpu_attention_decode_paged: DEVICE pointers unless a
  * comment says host, no engine handle, the call only enqueues work on cuda_stream (a
  * cudaStream_t; NULL = legacy default stream) of the calling thread's current device, on which
- * all pointers must be usable, and may be captured into a CUDA graph.  The descriptors are host
- * structs, read before the call returns.  Errors: non-zero return, message from
+ * all pointers must be usable, and may be captured into a CUDA graph (under lazy loading the first
+ * call of an op on a device loads its kernels: make that one outside a capture).  The descriptors
+ * are host structs, read before the call returns.  Errors: non-zero return, message from
  * mossgpu_op_last_error() (per thread); a refused call enqueues nothing.  Values that only the
  * device sees (row bounds, slots, positions, page ids, tokens) are checked there: what is out of
  * range is skipped and recorded for mossgpu_op_device_status: 9 = a slot or position outside the
@@ -344,7 +358,8 @@ typedef struct {
 
 /* A ragged batch: sequence s owns rows row_start[s] .. row_start[s + 1] - 1 of the row tensors
  * (row_start ascends; a sequence may own none), lives in slot[s] and has ctx_len[s] positions in
- * the cache already: its i-th row is position ctx_len[s] + i.  The slots of a call are distinct.
+ * the cache already: its i-th row is position ctx_len[s] + i.  The slots of a call are distinct, and
+ * the pages that an append writes belong to one slot alone (pages that are only read may be shared).
  * Rows outside every sequence are left as they are. */
 typedef struct {
     const int32_t *row_start;  /* [n_seqs + 1] */

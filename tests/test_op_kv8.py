@@ -358,6 +358,58 @@ def test_attention(M, L, lengths, use_mask, t, fmt, dim, kvh, group):
     assert torch.equal(again[: starts[-1]], out[: starts[-1]])
 
 
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("new,group", [(1, 1), (3, 4), (20, 4)])
+@pytest.mark.parametrize("scale", [0.0, -0.2])
+def test_attention_any_sign_of_the_scale(M, L, t, new, group, scale):
+    # the forms for few, some and many rows, each with and without a split over positions
+    for seqs_n in (2, 90):
+        lengths = [(new, 37 * (i % 3)) for i in range(seqs_n)]
+        starts, slots, ctx = layout(lengths)
+        cache = R.Cache(R.E4M3, 2, 64, seqs_n, 7, seed=3)
+        for s in range(min(seqs_n, 6)):
+            cache.fill(slots[s], ctx[s] + new, s)
+        for s in range(6, seqs_n):  # the others share the first ones' pages: they are read only
+            cache.table[slots[s]] = cache.table[slots[s % 6]]
+        q = torch.randn(starts[-1], 2 * group, 64, generator=torch.Generator().manual_seed(1)).to(t)
+        out = torch.empty_like(q, device="cuda")
+        keep, seqs = batch(M, starts, slots, ctx, starts[-1])
+        attend(M, L, cache.cuda(), seqs, q.cuda(), out, scale)
+        assert status(L) == 0
+        n = 6 if seqs_n > 6 else seqs_n
+        want, mass, top = R.attend64(cache, q[: starts[n]].double(), starts[: n + 1], slots[:n], ctx[:n], scale)
+        assert ((out[: starts[n]].cpu().double() - want).abs() <= R.attend_tolerance(mass, top, want, t)).all()
+        if seqs_n > 6:  # every later sequence has the cache and the context of one of the first six, but its own queries
+            for s in (6, 47, 89):
+                own = R.attend64(cache, q[starts[s] : starts[s + 1]].double(), [0, new], [slots[s]], [ctx[s]], scale)
+                assert ((out[starts[s] : starts[s + 1]].cpu().double() - own[0]).abs() <= R.attend_tolerance(own[1], own[2], own[0], t)).all()
+
+
+@pytest.mark.parametrize("dim,new,group,t", [(64, 1, 1, F32), (128, 1, 2, BF16), (64, 2, 3, F32), (128, 2, 8, BF16), (64, 3, 8, F16)])
+def test_attention_the_most_sequences(M, L, dim, new, group, t):
+    # 4096 sequences, some without rows, that all read a few slots' pages
+    n = 4096
+    lengths = [(0 if i % 7 == 3 else new, i % 50) for i in range(n)]
+    starts, slots, ctx = layout(lengths)
+    cache = R.Cache(R.INT8, 1, dim, n, 4, seed=3)
+    for s in range(50):
+        cache.fill(slots[s], 49 + new, s)
+    for s in range(50, n):
+        cache.table[slots[s]] = cache.table[slots[s % 50]]
+    q = torch.randn(starts[-1], group, dim, generator=torch.Generator().manual_seed(1)).to(t)
+    buf = torch.full((starts[-1] + 1, group, dim), SENTINEL, dtype=t, device="cuda")
+    keep, seqs = batch(M, starts, slots, ctx, starts[-1])
+    attend(M, L, cache.cuda(), seqs, q.cuda(), buf[: starts[-1]], dim**-0.5)
+    assert status(L) == 0 and (buf[-1] == SENTINEL).all()
+    got = buf[: starts[-1]].cpu().double()
+    assert torch.isfinite(got).all()
+    for s in list(range(0, n, 97)) + [n - 1]:
+        if starts[s + 1] > starts[s]:
+            rows = slice(starts[s], starts[s + 1])
+            want, mass, top = R.attend64(cache, q[rows].double(), [0, new], [slots[s]], [ctx[s]], float(np.float32(dim**-0.5)))
+            assert ((got[rows] - want).abs() <= R.attend_tolerance(mass, top, want, t)).all()
+
+
 def test_attention_misaligned_rows(M, L):
     # odd strides and a base off 16 bytes: element-wise loads and stores
     for t in R.TYPES:
@@ -539,3 +591,57 @@ def test_long_pool_offsets(M, L):
     want = torch.einsum("hij,jd->ihd", torch.softmax(s, -1), vb[:, 0].double())
     # the scores stay below 2^6 with |q||k| sums of that order: attend_tolerance gives under 1e-3 of max |v| (about 4)
     assert ((out.double() - want).abs() <= 2.5e-4).all()
+
+
+@pytest.mark.parametrize("fmt", [R.INT8, R.E4M3])
+@pytest.mark.parametrize("t", [F32, BF16])
+def test_prompt_draft_score_and_next_token(M, L, fmt, t):
+    # the operators as a server runs them, one layer: a prompt, a tree of drafted tokens that share rotary positions by
+    # depth, the drafts' log-probabilities, the accepted branch moved (read, appended again), one more token
+    import test_op_logprobs as P
+    kvh, group, dim, vocab, rot = 2, 3, 64, 777, 48
+    qh = kvh * group
+    g = torch.Generator().manual_seed(7)
+    cache = R.Cache(fmt, kvh, dim, 2, 6, seed=2)
+    dev = cache.cuda()
+    steps, mag = M.rope_steps(rot)
+    steps = torch.from_numpy(steps.view(np.int64)).cuda()
+    rope = M.Rope(steps.data_ptr(), rot, 0, mag)
+    head = torch.randn(qh * dim, vocab, generator=g).cuda()
+
+    def step(starts, ctx, mask=None, pos=None):
+        rows = starts[-1]
+        k, v, q = (torch.randn(rows, h, dim, generator=g).to(t).cuda() for h in (kvh, kvh, qh))
+        keep, seqs = batch(M, starts, [1, 0], ctx, rows)
+        pd = torch.tensor(pos, dtype=torch.int32).cuda() if pos is not None else None
+        md = mask.cuda() if mask is not None else None
+        out = torch.empty_like(q)
+        ok(L, L.mossgpu_kv8_append(dev.struct(M), seqs, rope, append_args(M, k, v, q, q, pd), stream()))
+        attend(M, L, dev, seqs, q, out, 0.125, md)
+        assert status(L) == 0
+        host = R.Cache.__new__(R.Cache)
+        host.__dict__.update(cache.__dict__)
+        host.codes, host.scales = dev.codes.cpu(), dev.scales.cpu()
+        want, mass, top = R.attend64(host, q.cpu().double(), starts, [1, 0], ctx, 0.125, mask)
+        assert ((out.cpu().double() - want).abs() <= R.attend_tolerance(mass, top, want, t)).all()
+        return out
+
+    step([0, 37, 60], [0, 0])                                   # prompts of 37 and 23
+    # drafts: 0 -> 1 -> 3, 0 -> 2 for the first, a chain of two for the second
+    mask = torch.tensor([[0b1], [0b11], [0b101], [0b1011], [0b1], [0b11]], dtype=torch.int32)
+    out = step([0, 4, 6], [37, 23], mask, [37, 38, 38, 39, 23, 24])
+    logits = (out.float().view(6, -1) @ head).contiguous()
+    drafted = torch.randint(0, vocab, (6,), generator=g, dtype=torch.int32)
+    P.check(logits.cpu(), drafted, 5, 1.0, P.run(M, logits, drafted.cuda(), 5))
+    # the first sequence accepts 0, 2: position 39 (draft 2) moves to 38, without another rounding of the codes' values
+    k1 = torch.empty(1, kvh, dim, device="cuda")
+    v1 = torch.empty_like(k1)
+    keep, seqs = batch(M, [0, 1], [1], [39], 1)
+    ok(L, L.mossgpu_kv8_read(dev.struct(M), seqs, M.KV8ReadArgs(k=k1.data_ptr(), v=v1.data_ptr(), k_row_stride=kvh * dim,
+                             k_head_stride=dim, v_row_stride=kvh * dim, v_head_stride=dim, type=0), stream()))
+    keep2, seqs = batch(M, [0, 1], [1], [38], 1)
+    ok(L, L.mossgpu_kv8_append(dev.struct(M), seqs, None, append_args(M, k1, v1), stream()))
+    assert status(L) == 0
+    page, was, now = int(cache.table[1, 2]), 39 - 32, 38 - 32
+    assert torch.equal(dev.codes[page, :, :, now], dev.codes[page, :, :, was])
+    step([0, 1, 2], [39, 25])                                   # the next token of both

@@ -180,3 +180,39 @@ def test_captured(M):
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(lp.cpu(), want["lp"]) and torch.equal(ids.cpu(), want["ids"])
+
+
+def test_engine_scores_a_frame(M, weights_path):
+    # teacher-forced codes, the step's own codes and alternatives under the frame's logits, 3 streams
+    eng = M.Engine(weights_path, max_streams=4, max_ctx=64)
+    sids = [eng.open() for _ in range(3)]
+    rng = np.random.default_rng(5)
+    for i, sid in enumerate(sids):
+        eng.fill_state_random(sid, 5 + 7 * i, i)
+        eng.generate_begin(sid, i)
+    p = M.SampleParams.make(greedy=True, repetition_penalty=1.2, min_frames=99)
+    for forced in (rng.integers(0, 1024, (3, 16)).astype(np.int32), None):
+        codes, stop, _, logits = eng.step(sids, p, forced=forced, want_logits=True)
+        assert not stop.any()
+        x = torch.from_numpy(logits.reshape(48, 1024))
+        for asked in (forced, None):
+            if asked is None:
+                asked_codes = codes
+            else:
+                asked_codes = asked.copy()
+                asked_codes[1, 3] = -1
+            lp, ent, ids, top = eng.frame_logprobs(3, None if asked is None else asked_codes, top_k=6, temperature=0.9)
+            o = {"lp": torch.from_numpy(lp.reshape(-1)), "ent": torch.from_numpy(ent.reshape(-1)),
+                 "ids": torch.from_numpy(ids.reshape(48, 6)), "top": torch.from_numpy(top.reshape(48, 6))}
+            check(x, torch.from_numpy(asked_codes.reshape(-1)), 6, 0.9, o)
+    lp, ent, ids, top = eng.frame_logprobs(3)
+    assert ids is None and top is None and (lp < 0).all() and (ent > 0).all()
+    bad = np.full((3, 16), 1024, np.int32)
+    for kw, text in ((dict(n=2), "number of streams"), (dict(n=3, codes=bad), "out of range"), (dict(n=3, top_k=33), "top_k"),
+                     (dict(n=3, temperature=0.0), "temperature")):
+        with pytest.raises(M.MossGpuError, match=text):
+            eng.frame_logprobs(**kw)
+    eng.step_frames(sids, p, 2)
+    with pytest.raises(M.MossGpuError, match="number of streams"):
+        eng.frame_logprobs(3)
+    eng.close()

@@ -51,7 +51,7 @@ def attn(M, **kw):
 CACHES = [(dict(codes=0), "NULL"), (dict(scales=0), "NULL"), (dict(page_table=0), "NULL"), (dict(codes=P + 8), "16-byte"),
           (dict(scales=P + 4), "16-byte"), (dict(page_table=P + 2), "aligned"), (dict(n_pages=0), "positive"),
           (dict(n_slots=-1), "positive"), (dict(pages_per_slot=0), "positive"), (dict(pages_per_slot=1 << 27), "2^26"),
-          (dict(kv_heads=0), "kv_heads"), (dict(head_dim=96), "head_dim"), (dict(format=2), "format")]
+          (dict(kv_heads=0), "kv_heads"), (dict(kv_heads=1025), "kv_heads"), (dict(head_dim=96), "head_dim"), (dict(format=2), "format")]
 BATCHES = [(dict(n_seqs=-1), "n_seqs"), (dict(n_seqs=4097), "n_seqs"), (dict(rows=-1), "rows"), (dict(row_start=0), "NULL"),
            (dict(slot=0), "NULL"), (dict(ctx_len=0), "NULL"), (dict(ctx_len=P + 1), "aligned")]
 
@@ -134,6 +134,9 @@ def test_attention_refusals(M, kw, text):
 def test_attention_refuses_what_its_plan_cannot_count(M):
     c = cache(M, pages_per_slot=1 << 26)
     refused(M, M.lib().mossgpu_attention_kv8(c, seqs(M, rows=1000), attn(M), None), "split the call")
+    wide = dict(q_heads=64, q_row_stride=4096, out_row_stride=4096, workspace_bytes=1 << 62)
+    refused(M, M.lib().mossgpu_attention_kv8(cache(M, kv_heads=1), seqs(M, rows=1 << 25), attn(M, **wide), None), "2^30")
+    refused(M, M.lib().mossgpu_attention_kv8(cache(M), seqs(M, rows=1 << 29), attn(M, **wide), None), "2^33")
 
 
 def test_workspace_bytes(M):
