@@ -6,15 +6,14 @@
 // new rows times the query heads of the group, so a cache byte serves all of them.  A unit's
 // positions come in tiles of 32 (two pages).  All tiles of one head, in order, are cut into equal
 // runs, one run of one head per warp of the grid: however ragged the batch is, every warp has the
-// same work.  The heads of a run go to neighbouring warps, since a page's heads lie side by side:
-// 512 long sequences take 372 us with every head's tiles in a warp of its own somewhere, as the pages'
-// address translations are then missed for every 1 KB block.  A warp that has a whole unit writes its
-// rows; a unit cut between warps leaves partial sums in the workspace, which k_attn_kv8_join (a
+// same work.  The heads of a run go to neighbouring warps, since a page's heads lie side by side (512
+// long sequences: 364 us against 372 with the runs of a head behind one another).  A warp that has a whole
+// unit writes its rows; a unit cut between warps leaves partial sums in the workspace, which k_attn_kv8_join (a
 // dependent launch) merges in a fixed order, so that a result does not depend on timing.
 //
 // A tile.  K, V and their scales of the pages (each contiguous) are copied to a stage of the warp's own
-// ring in shared memory, 16 bytes a lane (bulk copies of 1 KB need more instructions: they are issued
-// one lane after the other).  No barrier but the warp's own.  S = q K^T
+// ring in shared memory, 16 bytes a lane (339 us for those sequences against 362 with bulk copies of 1 KB,
+// which are issued one lane after the other).  No barrier but the warp's own.  S = q K^T
 // and o += w V are mma.sync m16n8k16 products in fp16, in which every 8-bit code is exact.  Which
 // element of the head dimension is the k-th of a product, and which position is the n-th, is free as
 // long as both operands agree.  Here a lane takes 16 consecutive codes of a K row, the same columns of
@@ -30,6 +29,10 @@
 // fp16 part (22 bits) that occupy rows g and g + 8 of the same product, 8 rows a product; since the
 // tensor cores truncate when they accumulate, such products start from zero every tile and are added
 // in fp32.  Statistics, sums and partials are fp32.
+//
+// Measured on one B200: 512 sequences of 256-4096 positions, 12 heads of 64, int8: 300 us (6.1 TB/s, 93%
+// of the measured copy rate) in short bursts, 333-340 us (84%) when repeated for seconds, as the card then
+// lowers its clocks: about 450 instructions a tile of 32 positions keep the schedulers 62% busy.
 #pragma once
 
 #include <type_traits>
@@ -750,7 +753,8 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
 }
 
 // Units of more rows.  A CTA's four warps take 8 or 16 of them each; a tile is read once for all of
-// them, and its codes are converted to fp16 once, each thread its share, a tile ahead of its use (the
+// them (64 rows of bf16 over an e4m3 cache of heads of 128: 175 TFLOP/s; three warps a scheduler wait for
+// one another's shared-memory reads, 56% of that pipe, and products, 27% of theirs), and its codes are converted to fp16 once, each thread its share, a tile ahead of its use (the
 // conversions are as many instructions as the rest of a tile's work).  The warps take their fragments
 // from the converted tile with ldmatrix; its 16-byte chunks are stored at chunk ^ (row % 8).  A run
 // belongs to a CTA.
@@ -1371,21 +1375,21 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
     }
 }
 
-// One warp per (row, query head): merges the partial sums of a unit that was cut, in the order of
-// its positions.
-template <int D>
+// Merges the partial sums of units that were cut, in the order of their positions.  JOB_WARPS warps a
+// (row, query head) take a share of its partials each, 32 at a time: the references first, one a lane, then
+// the sums, whose loads then wait for nothing.
+template <int D, int JOB_WARPS>
 __global__ void __launch_bounds__(256) k_attn_kv8_join(const __grid_constant__ AttnKv8 p) {
+    __shared__ float shares[JOB_WARPS > 1 ? JOB_WARPS : 1][D + 4];
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31;
-    const int64_t job = int64_t(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t job = JOB_WARPS > 1 ? int64_t(blockIdx.x) : int64_t(blockIdx.x) * 8 + warp;
     const int row = int(job / p.a.q_heads), qh = int(job - int64_t(row) * p.a.q_heads);
     if (row >= p.seqs.rows) return;
-    const int s = warp_upper_bound(p.seqs.row_start, p.seqs.n_seqs, row) - 1;
-    if (s < 0) return;
-    const RowRange rr = kv8_rows(__ldg(p.seqs.row_start + s), __ldg(p.seqs.row_start + s + 1), p.seqs.rows);
-    if (row >= rr.r1) return;
-    const int H = p.cache.kv_heads, head = qh / p.group;
-    const int x = (row - rr.r0) * p.group + (qh - head * p.group), block = x / p.tile_rows;
+    RowOwner owner;
+    if (!row_owner(p.seqs, row, row, row, owner)) return;
+    const int s = owner.seq, H = p.cache.kv_heads, head = qh / p.group;
+    const int x = (row - owner.r.r0) * p.group + (qh - head * p.group), block = x / p.tile_rows;
     const uint32_t before = __ldcg(p.plan + s), tiles = __ldcg(p.plan + p.seqs.n_seqs + 1 + s);
     const int64_t total = __ldcg(p.plan + p.seqs.n_seqs);
     const int used = runs_used(total, p.runs);
@@ -1397,29 +1401,71 @@ __global__ void __launch_bounds__(256) k_attn_kv8_join(const __grid_constant__ A
     float m = -INFINITY, l = 0.f, o[E];
 #pragma unroll
     for (int i = 0; i < E; ++i) o[i] = 0.f;
-    const size_t in_slot = size_t(x - block * p.tile_rows) * (D + 4);
     const size_t slot = size_t(p.part_rows) * (D + 4);
-#pragma unroll 4
-    for (int w = w0; w <= w1; ++w) {
-        const float *part = p.part + (size_t(w) * H + head) * 2 * slot + (w == w0 ? slot : 0) + in_slot;
-        float v[E];
-        if constexpr (E == 2) {
-            const float2 a = __ldcg(reinterpret_cast<const float2 *>(part) + lane);
-            v[0] = a.x, v[1] = a.y;
-        } else {
-            const float4 a = __ldcg(reinterpret_cast<const float4 *>(part) + lane);
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        }
-        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(part + D));
-        const float m_new = fmaxf(m, ml.x), ref = m_new == -INFINITY ? 0.f : m_new;
-        const float fa = ex2(m - ref), fb = ex2(ml.x - ref);
-        m = m_new;
-        l = l * fa + ml.y * fb;
+    const float *part = p.part + size_t(head) * 2 * slot + size_t(x - block * p.tile_rows) * (D + 4);
+    const auto at = [&](int w) { return part + size_t(w) * H * 2 * slot + (w == w0 ? slot : 0); };
+    const int share = JOB_WARPS > 1 ? (w1 - w0 + JOB_WARPS) / JOB_WARPS : w1 - w0 + 1;  // neighbouring partials of a warp
+    const int first = JOB_WARPS > 1 ? w0 + warp * share : w0, last = JOB_WARPS > 1 ? min(w1, first + share - 1) : w1;
+    for (int b = first; b <= last; b += 32) {
+        const int n = min(32, last - b + 1);
+        float2 ml = make_float2(-INFINITY, 0.f);
+        if (lane < n) ml = __ldcg(reinterpret_cast<const float2 *>(at(b + lane) + D));
+        float top = ml.x;
 #pragma unroll
-        for (int i = 0; i < E; ++i) o[i] = o[i] * fa + v[i] * fb;
+        for (int k = 16; k > 0; k >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, k));
+        const float m_new = fmaxf(m, top), ref = m_new == -INFINITY ? 0.f : m_new, old = ex2(m - ref), f = ex2(ml.x - ref);
+        m = m_new;
+        float sum = ml.y * f;
+#pragma unroll
+        for (int k = 16; k > 0; k >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, k);
+        l = fmaf(l, old, sum);
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] *= old;
+        for (int j0 = 0; j0 < n; j0 += 8) {
+            float v[8][E];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float *from = at(b + min(j0 + j, n - 1));
+                if constexpr (E == 2) {
+                    const float2 y = __ldcg(reinterpret_cast<const float2 *>(from) + lane);
+                    v[j][0] = y.x, v[j][1] = y.y;
+                } else {
+                    const float4 y = __ldcg(reinterpret_cast<const float4 *>(from) + lane);
+                    v[j][0] = y.x, v[j][1] = y.y, v[j][2] = y.z, v[j][3] = y.w;
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float fj = __shfl_sync(0xffffffffu, f, j0 + j);
+                if (j0 + j < n) {
+#pragma unroll
+                    for (int i = 0; i < E; ++i) o[i] = fmaf(v[j][i], fj, o[i]);
+                }
+            }
+        }
     }
-    const float f = l == 0.f ? 0.f : 1.f / l;
-    store_row<E>(p, row, qh, lane * E, o, f);
+    if constexpr (JOB_WARPS > 1) {
+#pragma unroll
+        for (int i = 0; i < E; ++i) shares[warp][lane * E + i] = o[i];
+        if (lane == 0) shares[warp][D] = m, shares[warp][D + 1] = l;
+        __syncthreads();
+        if (warp != 0) return;
+        m = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < JOB_WARPS; ++w) m = fmaxf(m, shares[w][D]);
+        const float ref = m == -INFINITY ? 0.f : m;
+        l = 0.f;
+#pragma unroll
+        for (int i = 0; i < E; ++i) o[i] = 0.f;
+#pragma unroll
+        for (int w = 0; w < JOB_WARPS; ++w) {
+            const float f = ex2(shares[w][D] - ref);
+            l = fmaf(shares[w][D + 1], f, l);
+#pragma unroll
+            for (int i = 0; i < E; ++i) o[i] = fmaf(shares[w][lane * E + i], f, o[i]);
+        }
+    }
+    store_row<E>(p, row, qh, lane * E, o, l == 0.f ? 0.f : 1.f / l);
 }
 
 }  // namespace mossgpu

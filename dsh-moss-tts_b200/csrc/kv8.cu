@@ -130,14 +130,21 @@ AttnForm attn_rows(int64_t rows_per_unit, bool direct) {
     using B = Ak8Block<D>;
     constexpr int kRows = Rows<D, MODE>::kRows;
     if (direct) return {k_attn_kv8<D, FORMAT, MODE, true>, S::kWarps, 1, S::kRing, kRows, 0};
-    if (rows_per_unit <= kRows) return {k_attn_kv8<D, FORMAT, MODE, false>, S::kWarps, 1, S::kRing, kRows, kNumSMs * S::kWarps};
+    // A warp a unit reads a tile again for every 8 or 16 rows, a CTA once for 32 or 64, but as long for few of
+    // them: 48 sequences of 700-8000 positions (us; warp, CTA): 20 rows 186, 251; 32 rows 197, 256; 48 rows 274,
+    // 290; 64 rows 361, 313; of 20-96 rows 386, 441.  Long blocks of rows are the CTA form's.
+    if (rows_per_unit <= 12 * kRows) return {k_attn_kv8<D, FORMAT, MODE, false>, S::kWarps, 1, S::kRing, kRows, kNumSMs * S::kWarps};
     return {k_attn_kv8_block<D, FORMAT, MODE>, B::kWarps, B::kCtas, B::kRing, B::kWarps * kRows, kNumSMs * B::kCtas};
 }
 
 template <int D, int FORMAT>
 AttnForm attn_form(int type, int64_t rows_per_unit, int64_t rows, int n_seqs, int kv_heads, int pages) {
-    // A CTA a unit where they fit the machine at once and no warp gets long: one launch.  (Tiles are 32 positions.)
-    const auto direct = [&](int tile_rows, int warps) { return (rows / tile_rows + n_seqs) * kv_heads <= kNumSMs && pages <= 2 * 8 * warps; };
+    // A CTA a unit (one launch) where that is few rounds of CTAs and no warp gets more than 8 tiles of 32
+    // positions.  Us, one launch against two, 12 heads of 64: one stream of 300 positions 6.9, 10.9; 8 x 1000 8.9,
+    // 16.8; 32 x 1000 (480 units) 21.1, 24.1; but 32 x 100-3000 29.1, 27.3, and one of 4000 17.0, 14.3.
+    const auto direct = [&](int tile_rows, int warps) { return (rows / tile_rows + n_seqs) * kv_heads <= 4 * kNumSMs && pages <= 2 * 8 * warps; };
+    // The form for 4 rows takes 8 in two units: 128 streams of 256-4096 positions, 12 kv heads (us, this form, the
+    // next): 4 rows 92.5, 107.6; 8 rows 153, 104; one row of 512 streams 300, 318.
     if (rows_per_unit <= 4) {
         using S = Ak8Few<D>;
         if (direct(4, S::kWarps)) return {k_attn_kv8_few<D, FORMAT, true>, S::kWarps, 1, S::kRing, 4, 0};
@@ -387,12 +394,17 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     at[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.gridDim = dim3(unsigned((jobs + 7) / 8));
+    // Few (row, head) pairs mean long units in many parts: a CTA each then (one stream of 4000 positions: the
+    // join alone 66 us with a warp each), a warp each otherwise.
+    const bool wide = jobs <= kNumSMs * 8;
+    cfg.gridDim = dim3(unsigned(wide ? jobs : (jobs + 7) / 8));
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     cfg.attrs = at;
     cfg.numAttrs = 1;
-    e = cache->head_dim == 64 ? cudaLaunchKernelEx(&cfg, k_attn_kv8_join<64>, p) : cudaLaunchKernelEx(&cfg, k_attn_kv8_join<128>, p);
+    const auto join = cache->head_dim == 64 ? (wide ? k_attn_kv8_join<64, 8> : k_attn_kv8_join<64, 1>)
+                                            : (wide ? k_attn_kv8_join<128, 8> : k_attn_kv8_join<128, 1>);
+    e = cudaLaunchKernelEx(&cfg, join, p);
     return e == cudaSuccess ? 0 : op_errorf("%s join launch: %s", who, cudaGetErrorString(e));
 }
 

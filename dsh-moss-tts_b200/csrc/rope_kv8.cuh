@@ -4,6 +4,9 @@
 // between.  Work goes to independent warps (no CTA barriers).  In k_rope_append LPH lanes (a power
 // of two) share a head, 8 elements a lane, and a warp takes several heads of one row: a lane has the
 // same columns in all of them, so its cosines and sines are computed once.
+// Measured on one B200: rotation of 8191 rows of 40 heads of 128 (bf16, half layout) 36.9 us, 4.5 TB/s; append
+// of 4232 rows of 32 + 8 + 8 such heads 30.7 us, 3.1 TB/s; read-back of 104,544 rows of 8 + 8 heads 117 us,
+// 5.6 TB/s (stores of whole 32-byte sectors: 138 us with two 16-byte ones a lane).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -317,7 +320,7 @@ struct RowOp {
 // The sequence that owns a row: its rows, slot and context.
 struct RowOwner {
     RowRange r;
-    int slot, ctx;
+    int seq, slot, ctx;
 };
 // Of rows first .. last (the same in the whole warp), each lane's own `row`.  32 neighbouring sequences
 // around where the rows would lie if all had as many are loaded at once, which finds them in one round
@@ -341,6 +344,7 @@ __device__ __forceinline__ bool row_owner(const mossgpu_seq_batch &q, int first,
             for (int j = 0; j < 32; ++j) s += __shfl_sync(0xffffffffu, start, j) <= row;
         }
         const int from = max(s, 0);
+        if (s >= 0) s += b0;
         start = __shfl_sync(0xffffffffu, start, from), end = __shfl_sync(0xffffffffu, end, from);
         slot = __shfl_sync(0xffffffffu, slot, from), ctx = __shfl_sync(0xffffffffu, ctx, from);
     } else {
@@ -353,7 +357,7 @@ __device__ __forceinline__ bool row_owner(const mossgpu_seq_batch &q, int first,
     }
     if (s < 0) return false;
     w.r = kv8_rows(start, end, q.rows);
-    w.slot = slot, w.ctx = ctx;
+    w.seq = s, w.slot = slot, w.ctx = ctx;
     return row >= w.r.r0 && row < w.r.r1;
 }
 
