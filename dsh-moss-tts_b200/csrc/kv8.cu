@@ -130,10 +130,10 @@ AttnForm attn_rows(int64_t rows_per_unit, bool direct) {
     using B = Ak8Block<D>;
     constexpr int kRows = Rows<D, MODE>::kRows;
     if (direct) return {k_attn_kv8<D, FORMAT, MODE, true>, S::kWarps, 1, S::kRing, kRows, 0};
-    // A warp a unit reads a tile again for every 8 or 16 rows, a CTA once for 32 or 64, but as long for few of
-    // them: 48 sequences of 700-8000 positions (us; warp, CTA): 20 rows 186, 251; 32 rows 197, 256; 48 rows 274,
-    // 290; 64 rows 361, 313; of 20-96 rows 386, 441.  Long blocks of rows are the CTA form's.
-    if (rows_per_unit <= 12 * kRows) return {k_attn_kv8<D, FORMAT, MODE, false>, S::kWarps, 1, S::kRing, kRows, kNumSMs * S::kWarps};
+    // A warp a unit reads and converts a tile again for every 8 or 16 rows, a CTA once for 32 or 64, but takes as
+    // long for few of them.  48 sequences of 700-8000 positions, 8 kv heads of 128, e4m3 (us when repeated for a
+    // second; warp, CTA): 20 rows 208, 253; 32 rows 219, 258; 48 rows 319, 294; 64 rows 404, 318; 96 rows 606, 554.
+    if (rows_per_unit <= 2 * kRows) return {k_attn_kv8<D, FORMAT, MODE, false>, S::kWarps, 1, S::kRing, kRows, kNumSMs * S::kWarps};
     return {k_attn_kv8_block<D, FORMAT, MODE>, B::kWarps, B::kCtas, B::kRing, B::kWarps * kRows, kNumSMs * B::kCtas};
 }
 
@@ -143,8 +143,9 @@ AttnForm attn_form(int type, int64_t rows_per_unit, int64_t rows, int n_seqs, in
     // positions.  Us, one launch against two, 12 heads of 64: one stream of 300 positions 6.9, 10.9; 8 x 1000 8.9,
     // 16.8; 32 x 1000 (480 units) 21.1, 24.1; but 32 x 100-3000 29.1, 27.3, and one of 4000 17.0, 14.3.
     const auto direct = [&](int tile_rows, int warps) { return (rows / tile_rows + n_seqs) * kv_heads <= 4 * kNumSMs && pages <= 2 * 8 * warps; };
-    // The form for 4 rows takes 8 in two units: 128 streams of 256-4096 positions, 12 kv heads (us, this form, the
-    // next): 4 rows 92.5, 107.6; 8 rows 153, 104; one row of 512 streams 300, 318.
+    // The form for 4 rows takes 8 in two units.  Streams of 256-4096 positions, 12 kv heads of 64, int8 (us when
+    // repeated for a second; this form, the next): one row of 512 streams 335, 380; 4 rows of 128 streams 96, 113; 8
+    // rows 177, 114.
     if (rows_per_unit <= 4) {
         using S = Ak8Few<D>;
         if (direct(4, S::kWarps)) return {k_attn_kv8_few<D, FORMAT, true>, S::kWarps, 1, S::kRing, 4, 0};
