@@ -31,7 +31,7 @@
 // in fp32.  Statistics, sums and partials are fp32.
 //
 // Measured on one B200: 512 sequences of 256-4096 positions, 12 heads of 64, int8: 300 us (6.1 TB/s, 93%
-// of the measured copy rate) in short bursts, 333-340 us (84%) when repeated for seconds, as the card then
+// of the measured copy rate) in short bursts, 323-343 us (81-86%) when repeated for seconds, as the card then
 // lowers its clocks: about 450 instructions a tile of 32 positions keep the schedulers 62% busy.
 #pragma once
 
