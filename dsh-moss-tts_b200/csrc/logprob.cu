@@ -256,34 +256,22 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
         }
     }
 
-    // ---- sums
-    float z = 0.f, s = 0.f;
+    // ---- sums.  x - M comes first: it is exact at the maximum and rounded relative to itself elsewhere, so that an
+    // exponent's error is within 2^-22 of the exponent whatever the sizes of the logits and of 1 / T are (x c - M c as one
+    // operation would leave half an ulp of M c in it)
     const float c = 1.4426950408889634f / a.temperature;
-    // (x - M) c as one operation where that cannot pass the range of fp32: its terms are relative to what
-    // M c rounds to, which the sums are corrected for
-    const float off = -top * c;
-    float miss = 0.f;  // by how much they are too large
-    if (fabsf(off) < 1e30f) {
-        miss = fmaf(top, c, off);
+    float z = 0.f, s = 0.f;
+    const float2 base = make_float2(-top, -top), c2 = make_float2(c, c);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            const uint4 y = vec(v);
+    for (int v = 0; v < NV; ++v) {
+        const uint4 y = vec(v);
 #pragma unroll
-            for (int i = 0; i < VE / 2; ++i) {
-                const float2 f = pair_of<T>(y, i);
-                const float t0 = fmaxf(fmaf(f.x, c, off), -200.f), t1 = fmaxf(fmaf(f.y, c, off), -200.f);
-                const float e0 = ex2(t0), e1 = ex2(t1);  // 2^-200 is 0, and 0 * infinity stays out of the sum
-                z += e0, s = fmaf(e0, t0, s);
-                z += e1, s = fmaf(e1, t1, s);
-            }
-        }
-    } else {
-#pragma unroll 1
-        for (int v = 0; v < NV * VE; ++v) {
-            const int id = id_of(v / VE, v % VE);
-            if (id < 0 || id >= a.vocab) continue;
-            const float t = fmaxf((float(x_row[id]) - top) * c, -200.f), e = ex2(t);
-            z += e, s = fmaf(e, t, s);
+        for (int i = 0; i < VE / 2; ++i) {
+            const float2 t = mul2(add2(pair_of<T>(y, i), base), c2);
+            // 2^-200 is 0, and 0 * infinity stays out of the sum; without a finite maximum NaN goes the same way
+            const float t0 = fmaxf(t.x, -200.f), t1 = fmaxf(t.y, -200.f), e0 = ex2(t0), e1 = ex2(t1);
+            z += e0, s = fmaf(e0, t0, s);
+            z += e1, s = fmaf(e1, t1, s);
         }
     }
 #pragma unroll
@@ -316,8 +304,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
             t.y += __shfl_xor_sync(0xffffffffu, t.y, o);
         }
         if (tid == 0) {
-            const float f = fmaf(-miss, kLpLn2, 1.f);  // 2^-miss
-            mine_part->top = top, mine_part->z = t.x * f, mine_part->s = fmaf(-miss, t.x, t.y) * f;
+            mine_part->top = top, mine_part->z = t.x, mine_part->s = t.y;
             mine_part->count = min(n, a.top_k);
         }
     }
