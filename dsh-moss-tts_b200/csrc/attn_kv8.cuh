@@ -197,7 +197,8 @@ __device__ __forceinline__ int run_of(int64_t total, int n, int64_t g) { return 
 __device__ __forceinline__ int runs_used(int64_t total, int runs) { return int(total < runs ? total : runs); }
 
 // Tiles (of TILE positions, over blocks of ROWS query rows, per kv head) before each sequence, in
-// shared memory, and, from CTA 0, in the workspace for k_attn_kv8_join.  Returns those of the batch.
+// shared memory, and, from CTA 0, in the workspace for k_attn_kv8_join.  Returns those of the batch, 0 where row
+// bounds that do not ascend make them too many to count.
 template <int ROWS, int TILE, int WARPS>
 __device__ __forceinline__ int64_t plan_tiles(const AttnKv8 &p, uint32_t *plan) {
     __shared__ uint32_t warp_sum[WARPS];
@@ -213,7 +214,7 @@ __device__ __forceinline__ int64_t plan_tiles(const AttnKv8 &p, uint32_t *plan) 
             if (r.r1 > r.r0) {
                 const SeqSpan span = kv8_span(p.cache, slot, ctx, r.r1 - r.r0, &status);
                 const uint32_t tiles = span.total > 0 ? (span.total + TILE - 1) / TILE : 1;
-                mine = tiles * uint32_t(((r.r1 - r.r0) * p.group + ROWS - 1) / ROWS);
+                mine = kv8_seq_tiles(tiles, r.r1 - r.r0, p.group, ROWS);
                 if (blockIdx.x == 0) p.plan[n_seqs + 1 + s] = tiles;
             }
             if (blockIdx.x == 0) op_report(p.status, status);
@@ -222,20 +223,26 @@ __device__ __forceinline__ int64_t plan_tiles(const AttnKv8 &p, uint32_t *plan) 
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const uint32_t v = __shfl_up_sync(0xffffffffu, sum, o);
-            if (lane >= o) sum += v;
+            if (lane >= o) sum = kv8_add_tiles(sum, v);
         }
         if (lane == 31) warp_sum[warp] = sum;
         __syncthreads();
         uint32_t base = before, all = 0;
         for (int w = 0; w < WARPS; ++w) {
-            if (w < warp) base += warp_sum[w];
-            all += warp_sum[w];
+            if (w < warp) base = kv8_add_tiles(base, warp_sum[w]);
+            all = kv8_add_tiles(all, warp_sum[w]);
         }
-        if (s < n_seqs) plan[s] = base + sum - mine;
-        before += all;
+        if (s < n_seqs) plan[s] = kv8_add_tiles(base, sum) - mine;
+        before = kv8_add_tiles(before, all);
         __syncthreads();
     }
-    if (threadIdx.x == 0) plan[n_seqs] = before;
+    if (threadIdx.x == 0) {
+        if (before == kKv8MaxTiles) {
+            before = 0;
+            if (blockIdx.x == 0) op_report(p.status, kStatusBadPosition);
+        }
+        plan[n_seqs] = before;
+    }
     __syncthreads();
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s <= n_seqs; s += WARPS * 32) p.plan[s] = plan[s];
@@ -1392,6 +1399,7 @@ __global__ void __launch_bounds__(256) k_attn_kv8_join(const __grid_constant__ A
     const int x = (row - owner.r.r0) * p.group + (qh - head * p.group), block = x / p.tile_rows;
     const uint32_t before = __ldcg(p.plan + s), tiles = __ldcg(p.plan + p.seqs.n_seqs + 1 + s);
     const int64_t total = __ldcg(p.plan + p.seqs.n_seqs);
+    if (total == 0) return;  // no plan
     const int used = runs_used(total, p.runs);
     const int64_t g0 = int64_t(before) + int64_t(block) * tiles, g1 = g0 + tiles;
     const int w0 = run_of(total, used, g0), w1 = run_of(total, used, g1 - 1);

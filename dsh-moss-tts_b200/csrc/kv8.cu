@@ -363,7 +363,7 @@ int mossgpu_attention_kv8(const mossgpu_kv8_cache *cache, const mossgpu_seq_batc
     if (int64_t(seqs->rows) * (g.q_heads / cache->kv_heads) > (1 << 30)) return op_errorf("%s: rows times heads of a group are above 2^30", who);
     // the plan counts tiles in 32 bits
     const int64_t blocks = int64_t(seqs->rows) * group / f.tile_rows + seqs->n_seqs;
-    if (blocks * (cache->pages_per_slot / 2 + 1) > INT64_C(0x7fffffff))
+    if (blocks * (cache->pages_per_slot / 2 + 1) >= int64_t(kKv8MaxTiles))
         return op_errorf("%s: rows times positions of the page table are above 2^31 tiles: split the call", who);
     int dev = -1, *status = nullptr;
     if (op_device(&dev, &status, who) != 0) return 1;

@@ -58,6 +58,20 @@ MOSSGPU_HD int kv8_page(const mossgpu_kv8_cache &c, int page, int *status) {
     return -1;
 }
 
+// Attention's plan counts tiles in 32 bits.  Row bounds that ascend keep a call's sum below kKv8MaxTiles, which the
+// host checks; bounds that do not (a row may then belong to many sequences) can pass it, so every sum stops there
+// instead of wrapping, and a plan that gets there is none.
+constexpr uint32_t kKv8MaxTiles = 0x7fffffffu;
+MOSSGPU_HD uint32_t kv8_add_tiles(uint32_t a, uint32_t b) {  // both at most kKv8MaxTiles
+    const uint32_t s = a + b;
+    return s < kKv8MaxTiles ? s : kKv8MaxTiles;
+}
+// Tiles of a sequence, `tiles` for each block of block_rows of its new rows times the heads of a group (at most 2^30).
+MOSSGPU_HD uint32_t kv8_seq_tiles(uint32_t tiles, int new_rows, int group, int block_rows) {
+    const uint64_t n = uint64_t(tiles) * uint32_t((new_rows * group + block_rows - 1) / block_rows);
+    return n < kKv8MaxTiles ? uint32_t(n) : kKv8MaxTiles;
+}
+
 // Element offsets: codes [n_pages][2][kv_heads][16][head_dim], scales [n_pages][2][kv_heads][16].
 MOSSGPU_HD size_t kv8_cell(const mossgpu_kv8_cache &c, int page, int half, int head, int off) {
     return ((size_t(page) * 2 + size_t(half)) * size_t(c.kv_heads) + size_t(head)) * kKv8Page + size_t(off);
