@@ -11,6 +11,8 @@
 namespace mossgpu {
 namespace {
 
+constexpr int kMaxHeads = 1 << 30;  // the kernels' head counters step past the last head by at most 2^18
+
 size_t type_size(int type) { return type == MOSSGPU_F32 ? 4 : 2; }
 bool is_type(int type) { return type >= MOSSGPU_F32 && type <= MOSSGPU_BF16; }
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
@@ -218,6 +220,7 @@ int mossgpu_rope_rotate(const mossgpu_rope *rope, const mossgpu_rope_args *args,
     if (!rope || !args) return op_errorf("%s: a descriptor is NULL", who);
     const mossgpu_rope_args &g = *args;
     if (g.rows < 0 || g.heads < 0) return op_errorf("%s: rows and heads must not be negative", who);
+    if (g.heads > kMaxHeads) return op_errorf("%s: heads = %d is above 2^30", who, g.heads);
     if (g.head_dim < 8 || g.head_dim > kMaxRopeDim || g.head_dim % 8)
         return op_errorf("%s: head_dim = %d must be a multiple of 8, 8 .. %d", who, g.head_dim, kMaxRopeDim);
     if (!is_type(g.type)) return op_errorf("%s: type %d is no element type", who, g.type);
@@ -260,6 +263,7 @@ int mossgpu_kv8_append(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *
     if (rope && check_rope(rope, cache->head_dim, who) != 0) return 1;
     if (g.q && !rope) return op_errorf("%s: q is given without a rope", who);
     if (g.q_heads < 0 || (g.q && g.q_heads == 0)) return op_errorf("%s: q_heads = %d", who, g.q_heads);
+    if (g.q_heads > kMaxHeads) return op_errorf("%s: q_heads = %d is above 2^30", who, g.q_heads);
     if (batch < 0) return 0;
     if (!g.k || !g.v || (g.q && !g.q_out)) return op_errorf("%s: a required pointer is NULL", who);
     const size_t size = type_size(g.type);

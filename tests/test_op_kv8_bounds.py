@@ -20,6 +20,17 @@ def test_plan_counts(tmp_path):
     assert r.returncode == 0, r.stdout + r.stderr
 
 
+def test_head_counts_at_the_end_of_their_type(M):
+    # counters that step by several heads would pass 2^31
+    import test_op_refusals as T
+    for heads in (2**31 - 1, 2**31 - 5, 2**30 + 1):
+        a = M.RopeArgs(x=T.P, out=2 * T.P, pos=T.P, x_row_stride=8, x_head_stride=0, out_row_stride=8, out_head_stride=8, rows=1,
+                       heads=heads, head_dim=8)
+        T.refused(M, M.lib().mossgpu_rope_rotate(T.rope(M, rotary_dim=8), a, None), "above 2^30")
+        a = T.append(M, q=T.P, q_out=2 * T.P, q_heads=heads, q_out_row_stride=64, q_out_head_stride=64)
+        T.refused(M, M.lib().mossgpu_kv8_append(T.cache(M), T.seqs(M, rows=1), T.rope(M), a, None), "above 2^30")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,t", [(8192, torch.float32), (65536, torch.bfloat16), (65536, torch.float16)])
 def test_rows_claimed_by_many_sequences(M, L, rows, t):
