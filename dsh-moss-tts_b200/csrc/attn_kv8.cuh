@@ -161,6 +161,15 @@ __device__ __forceinline__ void codes_f16(uint32_t w, uint32_t &lo, uint32_t &hi
 
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
 
+// A query row whose largest element is `top` enters the products times `to`, a power of two with the sign of the
+// scale that takes it to [128, 256) (elements below 2^-119 stay below that), and its products with K times `rf` are
+// scores in log2.
+__device__ __forceinline__ void query_factors(float top, float scale, float &to, float &rf) {
+    const int e = max(-119, int(__float_as_uint(top) >> 23) - 127);  // 128 for infinity and NaN: `to` is still a number
+    to = scale == 0.f ? 0.f : copysignf(pow2i(7 - e), scale);
+    rf = scale == 0.f ? 1.f : fabsf(scale) * pow2i(e - 7) * 1.4426950408889634f;
+}
+
 // 8 elements of a row of q, whatever its type
 __device__ __forceinline__ void load_q8(const void *q, int type, bool vec, int64_t at, float (&x)[8]) {
     if (type == MOSSGPU_F32)
@@ -429,9 +438,8 @@ __device__ __forceinline__ void load_rows(const AttnKv8 &p, const Unit &u, int f
             }
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
-        const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
-        w.rf[r] = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
+        float to;
+        query_factors(top, p.a.scale, to, w.rf[r]);
 #pragma unroll
         for (int c = 0; c < D / 64; ++c)
 #pragma unroll
@@ -878,9 +886,8 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                 }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
-                const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
-                rf[r] = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
+                float to;
+                query_factors(top, p.a.scale, to, rf[r]);
 #pragma unroll
                 for (int i = 0; i < D / 8; ++i) {
                     const float2 y = make_float2(v[i].x * to, v[i].y * to);
@@ -1170,9 +1177,8 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
                 }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            const int e = max(-110, min(110, int(__float_as_uint(top) >> 23) - 127));
-            const float to = p.a.scale == 0.f ? 0.f : copysignf(pow2i(7 - e), p.a.scale);
-            rf = p.a.scale == 0.f ? 1.f : fabsf(p.a.scale) * 1.4426950408889634f * pow2i(e - 7);
+            float to;
+            query_factors(top, p.a.scale, to, rf);
             rf = __shfl_sync(0xffffffffu, rf, t * 8);
 #pragma unroll
             for (int c = 0; c < kChunks; ++c)

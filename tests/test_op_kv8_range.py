@@ -125,69 +125,6 @@ def test_queries_and_v_scales_of_any_size(M, L, form, t, fmt, dim, size):
 
 @pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("t", R.TYPES)
-@pytest.mark.parametrize("scale", [1e-6, 1e-12, 1e-30, 1e-45])
-def test_zero_queries_at_any_scale(M, L, form, t, scale):
-    # every position that is seen weighs the same, and none that is not, however small the scale
-    cache, q, starts, slots, new, group = setup(form, R.INT8, 64, t)
-    q.zero_()
-    want, mass, top = exact(cache, q.double(), starts, slots, scale)
-    got = run(M, L, cache, q, starts, slots, scale)
-    assert ((got - want).abs() <= R.attend_tolerance(mass, top, want, t)).all()
-
-
-@pytest.mark.parametrize("form", list(FORMS))
-@pytest.mark.parametrize("t", [F32, BF16])
-@pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
-@pytest.mark.parametrize("scale", [2.0**8, -(2.0**12), 2.0**16, 1.7 * 2.0**20, 2.0**40, -(2.0**100)])
-def test_scores_of_any_size(M, L, form, t, fmt, dim, scale):
-    # Whole numbers throughout, so that scores are exact: a few positions share the largest and lie at least
-    # |scale| above all others, which leaves the mean of their V
-    cache, q, starts, slots, new, group = setup(form, fmt, dim, t)
-    cache.scales[:, 0] = 1.0
-    g = torch.Generator().manual_seed(8)
-    base = torch.randint(0, 2, (dim,), generator=g) * 2 - 1
-    small = torch.randint(-12, 13, (cache.pages, cache.kvh, R.PAGE, dim), generator=g)
-    peak = (base * 64).float()
-    code = (lambda x: x.to(torch.int8).view(torch.uint8)) if fmt == R.INT8 else (lambda x: x.float().to(torch.float8_e4m3fn).view(torch.uint8))
-    cache.codes[:, 0] = code(small)
-    for p in (5, 6, 700, 1989):  # of the long context; the short ones keep what they have
-        page, off = each_place(cache, slots[0], p)
-        cache.codes[page, 0, :, off] = code(peak)
-    times = torch.randint(1, 5, (q.shape[0], q.shape[1], 1), generator=g)
-    q = (base * times).to(t) * (1 if scale > 0 else -1)
-    long_rows = slice(0, new)
-    want, mass, _ = exact(cache, q.double(), starts, slots, scale)
-    v = cache.heads(slots[0], CTX[0], 1)[[5, 6, 700, 1989]].mean(0).repeat_interleave(group, 0)
-    assert ((want[long_rows] - v).abs() <= 1e-12 * mass[long_rows]).all()
-    got = run(M, L, cache, q, starts, slots, scale)
-    tol = tolerance(cache, q, want, mass, torch.zeros(q.shape[:2], dtype=torch.float64), starts, slots, t, group)
-    assert ((got - want).abs() <= tol).all()
-
-
-@pytest.mark.parametrize("form", list(FORMS))
-@pytest.mark.parametrize("t", R.TYPES)
-@pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
-@pytest.mark.parametrize("causal", [False, True])
-def test_hidden_v_scales_do_not_count(M, L, form, t, fmt, dim, causal):
-    # A drafted token with a V scale 2^45 above the others', which some rows see and others do not: the rows that do not
-    # are as exact as without it.  Outputs that hold such values pass the range of fp16: those rows go unread there.
-    cache, q, starts, slots, new, group = setup(form, fmt, dim, t)
-    hidden = new - 1 if causal else 0
-    for s, slot in enumerate(slots):
-        page, off = each_place(cache, slot, CTX[s] + hidden)
-        cache.scales[page, 1, :, off] *= 2.0**45
-    mask = None
-    if not causal:  # every row sees itself and, from the second on, the one before it unless that is the first
-        mask = torch.tensor([[1 << i | (1 << (i - 1) if i > 1 else 0)] for _ in CTX for i in range(new)], dtype=torch.int32)
-    want, mass, top = exact(cache, q.double(), starts, slots, 0.125, mask)
-    got = run(M, L, cache, q, starts, slots, 0.125, mask)
-    tol = tolerance(cache, q, want, mass, top, starts, slots, t, group, mask)
-    rows = torch.tensor([t != F16 or r % new != hidden for r in range(starts[-1])])
-    assert ((got - want).abs() <= tol)[rows].all()
-
-
-@pytest.mark.parametrize("form", list(FORMS))
-@pytest.mark.parametrize("t", R.TYPES)
 @pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
 @pytest.mark.parametrize("half", [0, 1])
 def test_nan_only_where_it_is_seen(M, L, form, t, fmt, dim, half):
