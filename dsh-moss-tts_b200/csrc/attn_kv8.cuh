@@ -35,6 +35,8 @@
 // lowers its clocks: about 450 instructions a tile of 32 positions keep the schedulers 62% busy.
 #pragma once
 
+#include <float.h>
+
 #include <type_traits>
 
 #include "f32x2.cuh"
@@ -163,11 +165,11 @@ __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) 
 
 // A query row whose largest element is `top` enters the products times `to`, a power of two with the sign of the
 // scale that takes it to [128, 256) (elements below 2^-119 stay below that), and its products with K times `rf` are
-// scores in log2.
+// scores in log2.  rf is finite and above 0, as 0 and infinity would make NaN of scores that are masked or 0.
 __device__ __forceinline__ void query_factors(float top, float scale, float &to, float &rf) {
     const int e = max(-119, int(__float_as_uint(top) >> 23) - 127);  // 128 for infinity and NaN: `to` is still a number
     to = scale == 0.f ? 0.f : copysignf(pow2i(7 - e), scale);
-    rf = scale == 0.f ? 1.f : fabsf(scale) * pow2i(e - 7) * 1.4426950408889634f;
+    rf = scale == 0.f ? 1.f : fminf(fmaxf(fabsf(scale) * pow2i(e - 7) * 1.4426950408889634f, __int_as_float(1)), FLT_MAX);
 }
 
 // 8 elements of a row of q, whatever its type

@@ -125,6 +125,18 @@ def test_queries_and_v_scales_of_any_size(M, L, form, t, fmt, dim, size):
 
 @pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("t", R.TYPES)
+@pytest.mark.parametrize("scale", [1e-6, 1e-12, 1e-30, 1e-45])
+def test_zero_queries_at_any_scale(M, L, form, t, scale):
+    # every position that is seen weighs the same, and none that is not, however small the scale
+    cache, q, starts, slots, new, group = setup(form, R.INT8, 64, t)
+    q.zero_()
+    want, mass, top = exact(cache, q.double(), starts, slots, scale)
+    got = run(M, L, cache, q, starts, slots, scale)
+    assert ((got - want).abs() <= R.attend_tolerance(mass, top, want, t)).all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("t", R.TYPES)
 @pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
 @pytest.mark.parametrize("half", [0, 1])
 def test_nan_only_where_it_is_seen(M, L, form, t, fmt, dim, half):
