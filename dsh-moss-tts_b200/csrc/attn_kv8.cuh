@@ -22,9 +22,9 @@
 // its score (K) and its weight (V) in fp32.
 //
 // Precision.  A query row is scaled by a power of two to [128, 256) and rounded to fp16, exact for
-// bf16 and fp16 inputs.  Weights are taken relative to R = m - (140 - E), m the running maximum of the
-// scores (in log2) and E the exponent of the largest V scale so far: w = 2^(s - R) sv < 2^14 fits
-// fp16 whatever the scales are.  For bf16 outputs w is rounded to fp16 (2^-11 against the output's
+// bf16 and fp16 inputs.  Weights are w = 2^(rf (s - m) + 140 - E) sv, s the scores without the row's factor rf, m
+// their running maximum and E the exponent of the largest V scale so far: w < 2^14 fits fp16 whatever the scales
+// are, and, since the difference comes before the factor, however large the scores are.  For bf16 outputs w is rounded to fp16 (2^-11 against the output's
 // 2^-8), 16 rows a product.  For fp32 and fp16 outputs q and w are split into an upper and a lower
 // fp16 part (22 bits) that occupy rows g and g + 8 of the same product, 8 rows a product; since the
 // tensor cores truncate when they accumulate, such products start from zero every tile and are added
@@ -77,7 +77,7 @@ struct AttnKv8 {
     int part_rows;   // rows a partial keeps
     int vec_q, vec_out;
     uint32_t *plan;  // [n_seqs + 1] tiles (over row blocks, per kv head) before a sequence; then [n_seqs] tiles of one block
-    float *part;     // [2 * runs * kv_heads][part_rows][head_dim + 4]: sums, then R and l
+    float *part;     // [2 * runs * kv_heads][part_rows][head_dim + 4]: sums, then their reference and l
     int *status;
 };
 
@@ -171,6 +171,15 @@ __device__ __forceinline__ void query_factors(float top, float scale, float &to,
     to = scale == 0.f ? 0.f : copysignf(pow2i(7 - e), scale);
     rf = scale == 0.f ? 1.f : fminf(fmaxf(fabsf(scale) * pow2i(e - 7) * 1.4426950408889634f, __int_as_float(1)), FLT_MAX);
 }
+
+// What scores are taken relative to, where their running maximum is m
+__device__ __forceinline__ float score_base(float m) { return m == -INFINITY ? 0.f : m; }
+// What earlier sums are multiplied by when the maximum goes from m0 to m and the V scales' exponent from E0 to E
+__device__ __forceinline__ float sums_factor(float m0, float m, float rf, float E0, float E) { return ex2(fmaf(m0 - score_base(m), rf, E0 - E)); }
+// Partial sums are kept relative to their maximum alone, which is stored in log2 (finite where there is any): sums
+// relative to `bias` - E times this
+__device__ __forceinline__ float part_factor(float E, int bias) { return pow2i(int(E) - bias); }
+__device__ __forceinline__ float part_reference(float m, float rf) { return m == -INFINITY ? m : fmaxf(fminf(m * rf, 0.5f * FLT_MAX), -0.5f * FLT_MAX); }
 
 // 8 elements of a row of q, whatever its type
 __device__ __forceinline__ void load_q8(const void *q, int type, bool vec, int64_t at, float (&x)[8]) {
@@ -365,7 +374,7 @@ __device__ __forceinline__ Unit direct_unit(const AttnKv8 &p, int index, int til
     return u;
 }
 
-// Where a CTA has a whole unit: its warps' sums, ROWS rows of D + 4 floats each (sums, R, l) at `part` +
+// Where a CTA has a whole unit: its warps' sums, ROWS rows of D + 4 floats each (sums, reference, l) at `part` +
 // warp * stride, to the output.
 template <int D, int WARPS>
 __device__ __forceinline__ void join_warps(const AttnKv8 &p, const Unit &u, int rows, const float *part, int stride) {
@@ -409,8 +418,8 @@ struct Rows {
     uint32_t q[D / 16][4];
     float rf[NR];            // what makes a product a score in log2, above 0
     int new_row[NR];         // which new row of the sequence; -1: none
-    float o[NJ][2 * NR], ref[NR], m[NR], l[NR];
-    int E;                   // biased exponent of the largest V scale so far (scales below 2^-87 lose bits of their weights)
+    float o[NJ][2 * NR], m[NR], l[NR];  // m: the largest score, without rf
+    float E;                 // biased exponent of the largest V scale so far (scales below 2^-87 lose bits of their weights)
 };
 
 // The query rows from `first` on as fragments; the sign of the scale goes into them.
@@ -456,9 +465,9 @@ __device__ __forceinline__ void load_rows(const AttnKv8 &p, const Unit &u, int f
                     w.q[c * 4 + j][2 + r] = pack2(b);
                 }
             }
-        w.m[r] = w.ref[r] = -INFINITY, w.l[r] = 0.f;
+        w.m[r] = -INFINITY, w.l[r] = 0.f;
     }
-    w.E = 40;
+    w.E = 40.f;
 #pragma unroll
     for (int j = 0; j < w.NJ; ++j)
 #pragma unroll
@@ -550,10 +559,11 @@ __device__ __forceinline__ void tile_rows(const AttnKv8 &p, const Unit &u, uint8
         }
     }
     // the running exponent of the V scales
+    const float E0 = w.E;
     {
         uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
         if (b >= 0x7f800000u || p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
-        w.E = max(w.E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+        w.E = fmaxf(w.E, float(__reduce_max_sync(0xffffffffu, b) >> 23));
     }
     float corr[NR];
     // softmax
@@ -563,17 +573,15 @@ __device__ __forceinline__ void tile_rows(const AttnKv8 &p, const Unit &u, uint8
                          fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        w.m[r] = fmaxf(w.m[r], mx * w.rf[r]);
-        const float now = w.m[r] == -INFINITY ? -INFINITY : w.m[r] - float(140 - w.E);
-        const float use = now == -INFINITY ? 0.f : now;  // what the weights are relative to
-        corr[r] = ex2(w.ref[r] - use);
-        w.ref[r] = now;
-        const float2 rf2 = make_float2(w.rf[r], w.rf[r]), off = make_float2(-use, -use);
+        const float m = fmaxf(w.m[r], mx), base = score_base(m), up = 140.f - w.E;
+        corr[r] = sums_factor(w.m[r], m, w.rf[r], E0, w.E);
+        w.m[r] = m;
+        const float2 base2 = make_float2(-base, -base), rf2 = make_float2(w.rf[r], w.rf[r]), up2 = make_float2(up, up);
         float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float2 &x = sv[i][r];
-            x = fma2(x, rf2, off);
+            x = fma2(add2(x, base2), rf2, up2);
             x.x = ex2(x.x), x.y = ex2(x.y);
             sum = add2(sum, x);
         }
@@ -658,7 +666,7 @@ __device__ __forceinline__ void tile_rows(const AttnKv8 &p, const Unit &u, uint8
     __syncwarp();
 }
 
-// A warp's rows (from `first` on) to the output where `part` is NULL, else as sums, R and l to part[row].
+// A warp's rows (from `first` on) to the output where `part` is NULL, else as sums, reference and l to part[row].
 // Lane (g, t) has of its rows the elements 2 NJ t .. in two runs of NJ.
 template <int D, int MODE>
 __device__ __forceinline__ void finish_rows(const AttnKv8 &p, const Unit &u, int first, float *part, Rows<D, MODE> &w) {
@@ -685,13 +693,14 @@ __device__ __forceinline__ void finish_rows(const AttnKv8 &p, const Unit &u, int
                 }
         } else {
             float *to = part + (row8 + r * 8) * (D + 4);
+            const float f = part_factor(w.E, 140);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
                 for (int j = 0; j < NJ; j += 4)
-                    *reinterpret_cast<float4 *>(to + t * (2 * NJ) + e * NJ + j) =
-                        make_float4(w.o[j][2 * r + e], w.o[j + 1][2 * r + e], w.o[j + 2][2 * r + e], w.o[j + 3][2 * r + e]);
-            if (t == 0) to[D] = w.ref[r], to[D + 1] = w.l[r];
+                    *reinterpret_cast<float4 *>(to + t * (2 * NJ) + e * NJ + j) = make_float4(
+                        w.o[j][2 * r + e] * f, w.o[j + 1][2 * r + e] * f, w.o[j + 2][2 * r + e] * f, w.o[j + 3][2 * r + e] * f);
+            if (t == 0) to[D] = part_reference(w.m[r], w.rf[r]), to[D + 1] = w.l[r] * f;
         }
     }
 }
@@ -823,6 +832,7 @@ template <int D, int FORMAT, int MODE>
 __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(const __grid_constant__ AttnKv8 p) {
     using S = Ak8Block<D>;
     constexpr int NR = MODE == kSplit ? 1 : 2, kWarpRows = 8 * NR, kRows = S::kWarps * kWarpRows, kBlock = 16 * D;
+    constexpr int kBias = MODE == kHalf ? 134 : 140;  // of the weights' exponents
     extern __shared__ __align__(16) uint8_t smem[];
     uint32_t *plan = reinterpret_cast<uint32_t *>(smem + S::kRing);
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -871,8 +881,8 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
             const int first = u.block * kRows + warp * kWarpRows;
             const bool any = first < u.n_rows;  // else the warp only copies and converts
             uint32_t q[D / 16][4];
-            float rf[NR], ref[NR], m[NR], l[NR], o[D / 8][2 * NR];
-            int new_row[NR], E = 40;
+            float rf[NR], m[NR], l[NR], o[D / 8][2 * NR], E = 40.f;
+            int new_row[NR];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
                 const int x = first + row8 + r * 8;
@@ -898,7 +908,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     else
                         q[i / 2][2 * (i & 1) + r] = pack2(y);
                 }
-                m[r] = ref[r] = -INFINITY, l[r] = 0.f;
+                m[r] = -INFINITY, l[r] = 0.f;
             }
 #pragma unroll
             for (int j = 0; j < D / 8; ++j)
@@ -982,10 +992,11 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                         }
                     }
                 }
+                const float E0 = E;
                 {
                     uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
                     if (b >= 0x7f800000u || (!whole && (p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)))) b = 0;
-                    E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+                    E = fmaxf(E, float(__reduce_max_sync(0xffffffffu, b) >> 23));
                 }
                 float corr[NR];
 #pragma unroll
@@ -994,24 +1005,22 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                                      fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    mx *= rf[r];
                     // kHalf: the reference follows the maximum only when that is 2^6 above it (weights stay below
                     // 2^14), as the sums have to be multiplied then
+                    const float m0 = m[r];
                     if constexpr (MODE == kHalf) {
-                        if (mx > m[r] + 6.f) m[r] = mx;
+                        if ((mx - m0) * rf[r] > 6.f) m[r] = mx;
                     } else {
-                        m[r] = fmaxf(m[r], mx);
+                        m[r] = fmaxf(m0, mx);
                     }
-                    const float now = m[r] == -INFINITY ? -INFINITY : m[r] - float((MODE == kHalf ? 134 : 140) - E);
-                    const float use = now == -INFINITY ? 0.f : now;
-                    corr[r] = ex2(ref[r] - use);
-                    ref[r] = now;
-                    const float2 rf2 = make_float2(rf[r], rf[r]), off = make_float2(-use, -use);
+                    const float base = score_base(m[r]), up = float(kBias) - E;
+                    corr[r] = sums_factor(m0, m[r], rf[r], E0, E);
+                    const float2 base2 = make_float2(-base, -base), rf2 = make_float2(rf[r], rf[r]), up2 = make_float2(up, up);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         float2 &x = sv[j][r];
-                        x = fma2(x, rf2, off);
+                        x = fma2(add2(x, base2), rf2, up2);
                         x.x = ex2(x.x), x.y = ex2(x.y);
                         sum = add2(sum, x);
                     }
@@ -1095,9 +1104,11 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     }
                 } else {
                     float *to = part + r * 8 * (D + 4);
+                    const float f = part_factor(E, kBias);
 #pragma unroll
-                    for (int j = 0; j < D / 8; ++j) *reinterpret_cast<float2 *>(to + 8 * j + 2 * t) = make_float2(o[j][2 * r], o[j][2 * r + 1]);
-                    if (t == 0) to[D] = ref[r], to[D + 1] = l[r];
+                    for (int j = 0; j < D / 8; ++j)
+                        *reinterpret_cast<float2 *>(to + 8 * j + 2 * t) = make_float2(o[j][2 * r] * f, o[j][2 * r + 1] * f);
+                    if (t == 0) to[D] = part_reference(m[r], rf[r]), to[D + 1] = l[r] * f;
                 }
             }
             run.g += t1 - t0;
@@ -1196,8 +1207,7 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
         const int x_row = u.block * 4 + t;
         const int new_row = x_row < u.n_rows ? x_row / p.group : -1;
 
-        float o[NO], ref = -INFINITY, m = -INFINITY, l = 0.f;
-        int E = 40;
+        float o[NO], m = -INFINITY, l = 0.f, E = 40.f;
 #pragma unroll
         for (int j = 0; j < NO; ++j) o[j] = 0.f;
 
@@ -1282,6 +1292,7 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
                 }
             }
             // the running exponent of the V scales
+            const float E0 = E;
             {
                 uint32_t b = 0;
 #pragma unroll
@@ -1291,7 +1302,7 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
                     if (v >= 0x7f800000u || (!whole && (p0 + r >= u.span.total || !(ok >> (r >> 4) & 1u)))) v = 0;
                     b = max(b, v);
                 }
-                E = max(E, int(__reduce_max_sync(0xffffffffu, b) >> 23));
+                E = fmaxf(E, float(__reduce_max_sync(0xffffffffu, b) >> 23));
             }
             // softmax over the lanes of equal t
             float mx = fmaxf(sv[0].x, sv[0].y);
@@ -1299,17 +1310,15 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
             for (int i = 1; i < NP; ++i) mx = fmaxf(mx, fmaxf(sv[i].x, sv[i].y));
 #pragma unroll
             for (int i = 4; i < 32; i <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, i));
-            m = fmaxf(m, mx * rf);
-            const float now = m == -INFINITY ? -INFINITY : m - float(140 - E);
-            const float use = now == -INFINITY ? 0.f : now;
-            const float corr = ex2(ref - use);
-            ref = now;
-            const float2 rf2 = make_float2(rf, rf), off = make_float2(-use, -use);
+            const float m0 = m;
+            m = fmaxf(m, mx);
+            const float corr = sums_factor(m0, m, rf, E0, E), base = score_base(m), up = 140.f - E;
+            const float2 base2 = make_float2(-base, -base), rf2 = make_float2(rf, rf), up2 = make_float2(up, up);
             float2 sum = make_float2(0.f, 0.f);
             uint32_t wb[NP][2];  // weights as the right operand
 #pragma unroll
             for (int pg = 0; pg < NP; ++pg) {
-                float2 x = fma2(sv[pg], rf2, off);
+                float2 x = fma2(add2(sv[pg], base2), rf2, up2);
                 x.x = ex2(x.x), x.y = ex2(x.y);
                 sum = add2(sum, x);
                 float2 w = mul2(x, make_float2(sc[NP * 16 + pg * 16 + mine], sc[NP * 16 + pg * 16 + mine + 8]));
@@ -1375,10 +1384,11 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
                 }
             } else {
                 float *to = part + t * (D + 4);
+                const float f = part_factor(E, 140);
 #pragma unroll
                 for (int j = 0; j < NO; j += 4)
-                    *reinterpret_cast<float4 *>(to + row8 * NO + j) = make_float4(o[j], o[j + 1], o[j + 2], o[j + 3]);
-                if (row8 == 0) to[D] = ref, to[D + 1] = l;
+                    *reinterpret_cast<float4 *>(to + row8 * NO + j) = make_float4(o[j] * f, o[j + 1] * f, o[j + 2] * f, o[j + 3] * f);
+                if (row8 == 0) to[D] = part_reference(m, rf), to[D + 1] = l * f;
             }
         }
         if (DIRECT) {

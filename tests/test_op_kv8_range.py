@@ -136,6 +136,35 @@ def test_zero_queries_at_any_scale(M, L, form, t, scale):
 
 
 @pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
+@pytest.mark.parametrize("scale", [2.0**8, -(2.0**12), 2.0**16, 1.7 * 2.0**20, 2.0**40, -(2.0**100)])
+def test_scores_of_any_size(M, L, form, t, fmt, dim, scale):
+    # Whole numbers throughout, so that scores are exact: a few positions share the largest and lie at least
+    # |scale| above all others, which leaves the mean of their V
+    cache, q, starts, slots, new, group = setup(form, fmt, dim, t)
+    cache.scales[:, 0] = 1.0
+    g = torch.Generator().manual_seed(8)
+    base = torch.randint(0, 2, (dim,), generator=g) * 2 - 1
+    small = torch.randint(-12, 13, (cache.pages, cache.kvh, R.PAGE, dim), generator=g)
+    peak = (base * 64).float()
+    code = (lambda x: x.to(torch.int8).view(torch.uint8)) if fmt == R.INT8 else (lambda x: x.float().to(torch.float8_e4m3fn).view(torch.uint8))
+    cache.codes[:, 0] = code(small)
+    for p in (5, 6, 700, 1989):  # of the long context; the short ones keep what they have
+        page, off = each_place(cache, slots[0], p)
+        cache.codes[page, 0, :, off] = code(peak)
+    times = torch.randint(1, 5, (q.shape[0], q.shape[1], 1), generator=g)
+    q = (base * times).to(t) * (1 if scale > 0 else -1)
+    long_rows = slice(0, new)
+    want, mass, _ = exact(cache, q.double(), starts, slots, scale)
+    v = cache.heads(slots[0], CTX[0], 1)[[5, 6, 700, 1989]].mean(0).repeat_interleave(group, 0)
+    assert ((want[long_rows] - v).abs() <= 1e-12 * mass[long_rows]).all()
+    got = run(M, L, cache, q, starts, slots, scale)
+    tol = tolerance(cache, q, want, mass, torch.zeros(q.shape[:2], dtype=torch.float64), starts, slots, t, group)
+    assert ((got - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("t", R.TYPES)
 @pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
 @pytest.mark.parametrize("half", [0, 1])
