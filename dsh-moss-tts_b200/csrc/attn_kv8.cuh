@@ -23,8 +23,8 @@
 //
 // Precision.  A query row is scaled by a power of two to [128, 256) and rounded to fp16, exact for
 // bf16 and fp16 inputs.  Weights are w = 2^(rf (s - m) + 140 - E) sv, s the scores without the row's factor rf, m
-// their running maximum and E the exponent of the largest V scale so far: w < 2^14 fits fp16 whatever the scales
-// are, and, since the difference comes before the factor, however large the scores are.  For bf16 outputs w is rounded to fp16 (2^-11 against the output's
+// their running maximum and E the exponent of the largest V scale that the row has seen: w < 2^14 fits fp16
+// whatever the scales are, and, since the difference comes before the factor, however large the scores are.  For bf16 outputs w is rounded to fp16 (2^-11 against the output's
 // 2^-8), 16 rows a product.  For fp32 and fp16 outputs q and w are split into an upper and a lower
 // fp16 part (22 bits) that occupy rows g and g + 8 of the same product, 8 rows a product; since the
 // tensor cores truncate when they accumulate, such products start from zero every tile and are added
@@ -180,6 +180,12 @@ __device__ __forceinline__ float sums_factor(float m0, float m, float rf, float 
 // relative to `bias` - E times this
 __device__ __forceinline__ float part_factor(float E, int bias) { return pow2i(int(E) - bias); }
 __device__ __forceinline__ float part_reference(float m, float rf) { return m == -INFINITY ? m : fmaxf(fminf(m * rf, 0.5f * FLT_MAX), -0.5f * FLT_MAX); }
+
+// The bits of a scale's size, 0 for infinity and NaN
+__device__ __forceinline__ uint32_t finite_bits(float scale) {
+    const uint32_t b = __float_as_uint(scale) & 0x7fffffffu;
+    return b < 0x7f800000u ? b : 0u;
+}
 
 // 8 elements of a row of q, whatever its type
 __device__ __forceinline__ void load_q8(const void *q, int type, bool vec, int64_t at, float (&x)[8]) {
@@ -419,7 +425,7 @@ struct Rows {
     float rf[NR];            // what makes a product a score in log2, above 0
     int new_row[NR];         // which new row of the sequence; -1: none
     float o[NJ][2 * NR], m[NR], l[NR];  // m: the largest score, without rf
-    float E;                 // biased exponent of the largest V scale so far (scales below 2^-87 lose bits of their weights)
+    float E[NR];             // biased exponents of the largest V scales they have seen (scales below 2^-87 lose bits of their weights)
 };
 
 // The query rows from `first` on as fragments; the sign of the scale goes into them.
@@ -465,9 +471,8 @@ __device__ __forceinline__ void load_rows(const AttnKv8 &p, const Unit &u, int f
                     w.q[c * 4 + j][2 + r] = pack2(b);
                 }
             }
-        w.m[r] = -INFINITY, w.l[r] = 0.f;
+        w.m[r] = -INFINITY, w.l[r] = 0.f, w.E[r] = 40.f;
     }
-    w.E = 40.f;
 #pragma unroll
     for (int j = 0; j < w.NJ; ++j)
 #pragma unroll
@@ -558,12 +563,25 @@ __device__ __forceinline__ void tile_rows(const AttnKv8 &p, const Unit &u, uint8
             }
         }
     }
-    // the running exponent of the V scales
-    const float E0 = w.E;
-    {
-        uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
-        if (b >= 0x7f800000u || p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)) b = 0;
-        w.E = fmaxf(w.E, float(__reduce_max_sync(0xffffffffu, b) >> 23));
+    // the running exponents of the V scales
+    float E0[NR];
+#pragma unroll
+    for (int r = 0; r < NR; ++r) E0[r] = w.E[r];
+    if (whole) {
+        const float e = float(__reduce_max_sync(0xffffffffu, finite_bits(sc[32 + lane])) >> 23);
+#pragma unroll
+        for (int r = 0; r < NR; ++r) w.E[r] = fmaxf(w.E[r], e);
+    } else {  // a row's are those that it sees
+#pragma unroll
+        for (int r = 0; r < NR; ++r) {
+            uint32_t b = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (seen[r] >> i & 1u) b = max(b, finite_bits(sc[32 + (i >> 2) * kKv8Page + 4 * t + (i & 3)]));
+            b = max(b, __shfl_xor_sync(0xffffffffu, b, 1));
+            b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
+            w.E[r] = fmaxf(w.E[r], float(b >> 23));
+        }
     }
     float corr[NR];
     // softmax
@@ -573,8 +591,8 @@ __device__ __forceinline__ void tile_rows(const AttnKv8 &p, const Unit &u, uint8
                          fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float m = fmaxf(w.m[r], mx), base = score_base(m), up = 140.f - w.E;
-        corr[r] = sums_factor(w.m[r], m, w.rf[r], E0, w.E);
+        const float m = fmaxf(w.m[r], mx), base = score_base(m), up = 140.f - w.E[r];
+        corr[r] = sums_factor(w.m[r], m, w.rf[r], E0[r], w.E[r]);
         w.m[r] = m;
         const float2 base2 = make_float2(-base, -base), rf2 = make_float2(w.rf[r], w.rf[r]), up2 = make_float2(up, up);
         float2 sum = make_float2(0.f, 0.f);
@@ -693,7 +711,7 @@ __device__ __forceinline__ void finish_rows(const AttnKv8 &p, const Unit &u, int
                 }
         } else {
             float *to = part + (row8 + r * 8) * (D + 4);
-            const float f = part_factor(w.E, 140);
+            const float f = part_factor(w.E[r], 140);
 #pragma unroll
             for (int e = 0; e < 2; ++e)
 #pragma unroll
@@ -881,7 +899,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
             const int first = u.block * kRows + warp * kWarpRows;
             const bool any = first < u.n_rows;  // else the warp only copies and converts
             uint32_t q[D / 16][4];
-            float rf[NR], m[NR], l[NR], o[D / 8][2 * NR], E = 40.f;
+            float rf[NR], m[NR], l[NR], E[NR], o[D / 8][2 * NR];
             int new_row[NR];
 #pragma unroll
             for (int r = 0; r < NR; ++r) {
@@ -908,7 +926,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     else
                         q[i / 2][2 * (i & 1) + r] = pack2(y);
                 }
-                m[r] = -INFINITY, l[r] = 0.f;
+                m[r] = -INFINITY, l[r] = 0.f, E[r] = 40.f;
             }
 #pragma unroll
             for (int j = 0; j < D / 8; ++j)
@@ -992,11 +1010,24 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                         }
                     }
                 }
-                const float E0 = E;
-                {
-                    uint32_t b = __float_as_uint(sc[32 + lane]) & 0x7fffffffu;
-                    if (b >= 0x7f800000u || (!whole && (p0 + lane >= u.span.total || !(ok >> (lane >> 4) & 1u)))) b = 0;
-                    E = fmaxf(E, float(__reduce_max_sync(0xffffffffu, b) >> 23));
+                float E0[NR];
+#pragma unroll
+                for (int r = 0; r < NR; ++r) E0[r] = E[r];
+                if (whole) {
+                    const float e = float(__reduce_max_sync(0xffffffffu, finite_bits(sc[32 + lane])) >> 23);
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) E[r] = fmaxf(E[r], e);
+                } else {  // a row's are those that it sees
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        uint32_t b = 0;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            if (seen[r] >> i & 1u) b = max(b, finite_bits(sc[32 + 8 * (i >> 1) + 2 * t + (i & 1)]));
+                        b = max(b, __shfl_xor_sync(0xffffffffu, b, 1));
+                        b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
+                        E[r] = fmaxf(E[r], float(b >> 23));
+                    }
                 }
                 float corr[NR];
 #pragma unroll
@@ -1013,8 +1044,8 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     } else {
                         m[r] = fmaxf(m0, mx);
                     }
-                    const float base = score_base(m[r]), up = float(kBias) - E;
-                    corr[r] = sums_factor(m0, m[r], rf[r], E0, E);
+                    const float base = score_base(m[r]), up = float(kBias) - E[r];
+                    corr[r] = sums_factor(m0, m[r], rf[r], E0[r], E[r]);
                     const float2 base2 = make_float2(-base, -base), rf2 = make_float2(rf[r], rf[r]), up2 = make_float2(up, up);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -1104,7 +1135,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     }
                 } else {
                     float *to = part + r * 8 * (D + 4);
-                    const float f = part_factor(E, kBias);
+                    const float f = part_factor(E[r], kBias);
 #pragma unroll
                     for (int j = 0; j < D / 8; ++j)
                         *reinterpret_cast<float2 *>(to + 8 * j + 2 * t) = make_float2(o[j][2 * r] * f, o[j][2 * r + 1] * f);
@@ -1291,18 +1322,22 @@ __global__ void __launch_bounds__(Ak8Few<D>::kWarps * 32, 1) k_attn_kv8_few(cons
                     if (!in) ((i & 1) ? sv[i >> 1].y : sv[i >> 1].x) = -INFINITY;
                 }
             }
-            // the running exponent of the V scales
+            // the running exponent of the V scales, of row t
             const float E0 = E;
             {
                 uint32_t b = 0;
+                if (whole) {
 #pragma unroll
-                for (int k = 0; k < NP / 2; ++k) {
-                    const int r = lane + 32 * k;
-                    uint32_t v = __float_as_uint(sc[NP * 16 + r]) & 0x7fffffffu;
-                    if (v >= 0x7f800000u || (!whole && (p0 + r >= u.span.total || !(ok >> (r >> 4) & 1u)))) v = 0;
-                    b = max(b, v);
+                    for (int k = 0; k < NP / 2; ++k) b = max(b, finite_bits(sc[NP * 16 + lane + 32 * k]));
+                    b = __reduce_max_sync(0xffffffffu, b);
+                } else {  // of what it sees
+#pragma unroll
+                    for (int i = 0; i < 2 * NP; ++i)
+                        if (seen >> i & 1u) b = max(b, finite_bits(sc[NP * 16 + (i >> 1) * kKv8Page + mine + 8 * (i & 1)]));
+#pragma unroll
+                    for (int i = 4; i < 32; i <<= 1) b = max(b, __shfl_xor_sync(0xffffffffu, b, i));
                 }
-                E = fmaxf(E, float(__reduce_max_sync(0xffffffffu, b) >> 23));
+                E = fmaxf(E, float(b >> 23));
             }
             // softmax over the lanes of equal t
             float mx = fmaxf(sv[0].x, sv[0].y);

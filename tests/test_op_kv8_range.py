@@ -167,6 +167,28 @@ def test_scores_of_any_size(M, L, form, t, fmt, dim, scale):
 @pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("t", R.TYPES)
 @pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_hidden_v_scales_do_not_count(M, L, form, t, fmt, dim, causal):
+    # A drafted token with a V scale 2^45 above the others', which some rows see and others do not: the rows that do not
+    # are as exact as without it.  Outputs that hold such values pass the range of fp16: those rows go unread there.
+    cache, q, starts, slots, new, group = setup(form, fmt, dim, t)
+    hidden = new - 1 if causal else 0
+    for s, slot in enumerate(slots):
+        page, off = each_place(cache, slot, CTX[s] + hidden)
+        cache.scales[page, 1, :, off] *= 2.0**45
+    mask = None
+    if not causal:  # every row sees itself and, from the second on, the one before it unless that is the first
+        mask = torch.tensor([[1 << i | (1 << (i - 1) if i > 1 else 0)] for _ in CTX for i in range(new)], dtype=torch.int32)
+    want, mass, top = exact(cache, q.double(), starts, slots, 0.125, mask)
+    got = run(M, L, cache, q, starts, slots, 0.125, mask)
+    tol = tolerance(cache, q, want, mass, top, starts, slots, t, group, mask)
+    rows = torch.tensor([t != F16 or r % new != hidden for r in range(starts[-1])])
+    assert ((got - want).abs() <= tol)[rows].all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("t", R.TYPES)
+@pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
 @pytest.mark.parametrize("half", [0, 1])
 def test_nan_only_where_it_is_seen(M, L, form, t, fmt, dim, half):
     # NaN scales at a context position of the second sequence, and at the first draft of the first, which the odd rows see
