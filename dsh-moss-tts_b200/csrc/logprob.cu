@@ -40,7 +40,7 @@ namespace cg = cooperative_groups;
 constexpr int kLpMaxTop = 32;
 constexpr int kLpMaxCluster = 16;
 constexpr int kLpMaxVocab = 500000;
-constexpr float kLpLn2 = 0.6931471805599453f;
+constexpr float kLpLn2 = 0.6931471805599453f, kLpLog2e = 1.4426950408889634f;
 
 struct LpPart {   // what a CTA of a cluster hands to rank 0
     float top, z, s;
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
     // ---- sums.  x - M comes first: it is exact at the maximum and rounded relative to itself elsewhere, so that an
     // exponent's error is within 2^-22 of the exponent whatever the sizes of the logits and of 1 / T are (x c - M c as one
     // operation would leave half an ulp of M c in it)
-    const float c = 1.4426950408889634f / a.temperature;
+    const float c = kLpLog2e / a.temperature;
     float z = 0.f, s = 0.f;
     const float2 base = make_float2(-top, -top), c2 = make_float2(c, c);
 #pragma unroll
@@ -455,8 +455,8 @@ extern "C" int mossgpu_token_logprobs(const mossgpu_logprob_args *args, void *cu
     if (a.type < MOSSGPU_F32 || a.type > MOSSGPU_BF16) return op_errorf("%s: type %d is no element type", who, a.type);
     if (a.top_k < 0 || a.top_k > kLpMaxTop || a.top_k > a.vocab)
         return op_errorf("%s: top_k = %d must be 0 .. min(%d, vocab)", who, a.top_k, kLpMaxTop);
-    if (!(a.temperature > 0.f) || !(a.temperature < INFINITY) || !(1.f / a.temperature < INFINITY))
-        return op_errorf("%s: temperature must be positive, and it and its inverse finite", who);
+    if (!(a.temperature > 0.f) || !(a.temperature < INFINITY) || !(kLpLog2e / a.temperature < INFINITY))
+        return op_errorf("%s: temperature must be positive, and it and log2(e) / temperature finite", who);
     if (a.rows > 1 && a.row_stride < a.vocab) return op_errorf("%s: row_stride is below vocab", who);
     if (a.rows == 0) return 0;
     if (!a.logits) return op_errorf("%s: logits is NULL", who);

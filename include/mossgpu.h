@@ -437,7 +437,7 @@ typedef struct {
     int rows, vocab;        /* vocab up to 500000 */
     int type;               /* of the logits */
     int top_k;              /* 0 .. min(32, vocab) */
-    float temperature;      /* > 0 */
+    float temperature;      /* > 0, large enough for log2(e) / temperature to be finite (4.3e-39) */
 } mossgpu_logprob_args;
 int mossgpu_token_logprobs(const mossgpu_logprob_args *args, void *cuda_stream);
 

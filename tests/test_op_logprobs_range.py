@@ -41,3 +41,14 @@ def test_large_16_bit_logits(M, t, scale, rows, vocab):
     x, _, tok = logits(rows, vocab, torch.float32, 13)
     x = (x.clamp(-4, 4) * scale).to(t)
     check(x, tok, 5, 0.7, run(M, x.cuda(), tok.cuda(), 5, 0.7))
+
+
+def test_temperatures_that_are_refused(M):
+    # 1 / T is finite and log2(e) / T is not: the maximum's own term would be 0 times infinity
+    L = M.lib()
+    for t in (3e-39, 4.2e-39, 1e-45):
+        a = M.LogprobArgs(logits=1 << 20, entropy=1 << 20, row_stride=100, rows=2, vocab=100, temperature=t)
+        assert L.mossgpu_token_logprobs(a, None) != 0 and b"temperature" in L.mossgpu_op_last_error()
+    x = torch.zeros(1, 100, device="cuda")
+    o = run(M, x, torch.zeros(1, dtype=torch.int32, device="cuda"), 1, 4.3e-39)
+    assert abs(o["lp"][0] + torch.log(torch.tensor(100.0))) < 1e-5 and o["top"][0, 0] == o["lp"][0]
