@@ -331,7 +331,12 @@ __global__ void __launch_bounds__(NT, NT == 32 ? 32 : 1024 / NT) k_token_logprob
     const bool empty = m == -INFINITY, bad = !(m < INFINITY);  // NaN or +inf
     const float log_z = log2f(zz), ln_z = log_z * kLpLn2, inv_t = 1.f / a.temperature, nan = __int_as_float(0x7fffffff);
     // (v - m) / T rather than ln 2 t: t of the type's lowest value is past the range of fp32
-    const auto logprob = [&](float v) { return bad ? nan : v == -INFINITY ? -INFINITY : (v - m) * inv_t - ln_z; };
+    // (and where v - m is past it as well, a high temperature may bring it back)
+    const auto logprob = [&](float v) {
+        if (bad || v == -INFINITY) return bad ? nan : v;
+        const float d = v - m;
+        return (d == -INFINITY ? fmaf(v, inv_t, -m * inv_t) : d * inv_t) - ln_z;
+    };
     if (tid == 0) {
         if (a.logprob) {
             const int t = __ldg(a.tokens + row);

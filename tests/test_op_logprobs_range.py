@@ -52,3 +52,15 @@ def test_temperatures_that_are_refused(M):
     x = torch.zeros(1, 100, device="cuda")
     o = run(M, x, torch.zeros(1, dtype=torch.int32, device="cuda"), 1, 4.3e-39)
     assert abs(o["lp"][0] + torch.log(torch.tensor(100.0))) < 1e-5 and o["top"][0, 0] == o["lp"][0]
+
+
+@pytest.mark.parametrize("rows,vocab", FORMS)
+@pytest.mark.parametrize("t", [torch.float32, torch.bfloat16])
+def test_lowest_value_below_large_logits(M, rows, vocab, t):
+    # the distance to the maximum passes the range of fp32, its quotient by the temperature does not
+    x, _, tok = logits(rows, vocab, torch.float32, 14)
+    x = (x.clamp(0, 9) * 1e37).to(t)
+    x[:, :3] = torch.finfo(t).min
+    x[:, 3] = 3e38
+    tok[:] = torch.arange(rows) % 4
+    check(x, tok, 5, 8.0, run(M, x.cuda(), tok.cuda(), 5, 8.0))
