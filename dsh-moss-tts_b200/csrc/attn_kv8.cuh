@@ -1010,13 +1010,10 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                         }
                     }
                 }
-                float E0[NR];
-#pragma unroll
-                for (int r = 0; r < NR; ++r) E0[r] = E[r];
+                // the tile's largest V scale, as its exponent, and its largest score, of each row
+                float e[NR], mx[NR];
                 if (whole) {
-                    const float e = float(__reduce_max_sync(0xffffffffu, finite_bits(sc[32 + lane])) >> 23);
-#pragma unroll
-                    for (int r = 0; r < NR; ++r) E[r] = fmaxf(E[r], e);
+                    e[0] = e[NR - 1] = float(__reduce_max_sync(0xffffffffu, finite_bits(sc[32 + lane])) >> 23);
                 } else {  // a row's are those that it sees
 #pragma unroll
                     for (int r = 0; r < NR; ++r) {
@@ -1026,26 +1023,47 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                             if (seen[r] >> i & 1u) b = max(b, finite_bits(sc[32 + 8 * (i >> 1) + 2 * t + (i & 1)]));
                         b = max(b, __shfl_xor_sync(0xffffffffu, b, 1));
                         b = max(b, __shfl_xor_sync(0xffffffffu, b, 2));
-                        E[r] = fmaxf(E[r], float(b >> 23));
+                        e[r] = float(b >> 23);
                     }
                 }
-                float corr[NR];
 #pragma unroll
                 for (int r = 0; r < NR; ++r) {
-                    float mx = fmaxf(fmaxf(fmaxf(sv[0][r].x, sv[0][r].y), fmaxf(sv[1][r].x, sv[1][r].y)),
-                                     fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-                    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    // kHalf: the reference follows the maximum only when that is 2^6 above it (weights stay below
-                    // 2^14), as the sums have to be multiplied then
-                    const float m0 = m[r];
-                    if constexpr (MODE == kHalf) {
-                        if ((mx - m0) * rf[r] > 6.f) m[r] = mx;
-                    } else {
-                        m[r] = fmaxf(m0, mx);
+                    mx[r] = fmaxf(fmaxf(fmaxf(sv[0][r].x, sv[0][r].y), fmaxf(sv[1][r].x, sv[1][r].y)),
+                                  fmaxf(fmaxf(sv[2][r].x, sv[2][r].y), fmaxf(sv[3][r].x, sv[3][r].y)));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 1));
+                    mx[r] = fmaxf(mx[r], __shfl_xor_sync(0xffffffffu, mx[r], 2));
+                }
+                // What the weights are relative to.  kHalf: m follows the maximum only when that is 2^6 above it (weights
+                // stay below 2^14), as the sums, which stay in the products' accumulators, have to be multiplied then;
+                // most tiles move nothing.
+                float corr[NR];
+                const auto follow = [&](int r, float m1) {
+                    const float E1 = fmaxf(E[r], e[r]);
+                    corr[r] = sums_factor(m[r], m1, rf[r], E[r], E1);
+                    m[r] = m1, E[r] = E1, l[r] *= corr[r];
+                };
+                if constexpr (MODE == kHalf) {
+                    bool above[NR], moves = false;
+#pragma unroll
+                    for (int r = 0; r < NR; ++r) {
+                        above[r] = (mx[r] - m[r]) * rf[r] > 6.f;
+                        moves = moves || above[r] || e[r] > E[r];
                     }
+                    if (__any_sync(0xffffffffu, moves)) {
+#pragma unroll
+                        for (int r = 0; r < NR; ++r) follow(r, above[r] ? mx[r] : m[r]);
+#pragma unroll
+                        for (int j = 0; j < D / 8; ++j) {
+                            o[j][0] *= corr[0], o[j][1] *= corr[0];
+                            o[j][2 * NR - 2] *= corr[NR - 1], o[j][2 * NR - 1] *= corr[NR - 1];
+                        }
+                    }
+                } else {
+                    follow(0, fmaxf(m[0], mx[0]));
+                }
+#pragma unroll
+                for (int r = 0; r < NR; ++r) {
                     const float base = score_base(m[r]), up = float(kBias) - E[r];
-                    corr[r] = sums_factor(m0, m[r], rf[r], E0[r], E[r]);
                     const float2 base2 = make_float2(-base, -base), rf2 = make_float2(rf[r], rf[r]), up2 = make_float2(up, up);
                     float2 sum = make_float2(0.f, 0.f);
 #pragma unroll
@@ -1055,7 +1073,7 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                         x.x = ex2(x.x), x.y = ex2(x.y);
                         sum = add2(sum, x);
                     }
-                    l[r] = fmaf(l[r], corr[r], sum.x + sum.y);
+                    l[r] += sum.x + sum.y;
                 }
                 uint32_t wa[2][4];  // the weights as the left operand, 16 positions each
                 const auto weights = [&](auto masked) {
@@ -1080,16 +1098,6 @@ __global__ void __launch_bounds__(128, Ak8Block<D>::kCtas) k_attn_kv8_block(cons
                     }
                 };
                 if (whole) weights(std::false_type()); else weights(std::true_type());
-                if constexpr (MODE == kHalf) {
-                    // the sums stay in the products' accumulators; most tiles raise no maximum
-                    if (__any_sync(0xffffffffu, corr[0] != 1.f || corr[NR - 1] != 1.f)) {
-#pragma unroll
-                        for (int j = 0; j < D / 8; ++j) {
-                            o[j][0] *= corr[0], o[j][1] *= corr[0];
-                            o[j][2 * NR - 2] *= corr[NR - 1], o[j][2 * NR - 1] *= corr[NR - 1];
-                        }
-                    }
-                }
                 const uint32_t v_s = tile_s + (32 + (lane & 15)) * (2 * D);  // the lane's row of the first 16
 #pragma unroll
                 for (int j = 0; j < D / 16; ++j) {  // 16 columns
