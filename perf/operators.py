@@ -375,7 +375,7 @@ def package():
 def descriptors(s):
     """The argument structs over this state's buffers; a program keeps them as it keeps the buffers."""
     M, c, op = package(), s["case"], s["case"]["op"]
-    d = {"lib": M.lib(), "stream": torch.cuda.current_stream().cuda_stream}
+    d = {"lib": M.lib()}
     kind = CTYPE[c["type"]]
     if "steps" in s:
         d["rope"] = M.Rope(s["steps"].data_ptr(), c["rot"], int(c["inter"]), s["mag"])
@@ -426,19 +426,20 @@ def run(s):
     c, op = s["case"], s["case"]["op"]
     if own:
         d = s.get("own") or s.setdefault("own", descriptors(s))
+        stream = torch.cuda.current_stream().cuda_stream  # of this pass: a later one may run on another
         if op == "rope":
-            called(d, d["lib"].mossgpu_rope_rotate(d["rope"], d["args"], d["stream"]))
+            called(d, d["lib"].mossgpu_rope_rotate(d["rope"], d["args"], stream))
             return s["out"]
         if op == "score":
-            called(d, d["lib"].mossgpu_token_logprobs(d["args"], d["stream"]))
+            called(d, d["lib"].mossgpu_token_logprobs(d["args"], stream))
             return {"logprob": s["lp"], "entropy": s["ent"], "top_ids": s["ids"], "top_logprobs": s["top"]}
         if op == "attend":
-            called(d, d["lib"].mossgpu_attention_kv8(d["cache"], d["seqs"], d["args"], d["stream"]))
+            called(d, d["lib"].mossgpu_attention_kv8(d["cache"], d["seqs"], d["args"], stream))
             return s["out"]
         if op != "read":
-            called(d, d["lib"].mossgpu_kv8_append(d["cache"], d["seqs"], d["rope"], d["append"], d["stream"]))
+            called(d, d["lib"].mossgpu_kv8_append(d["cache"], d["seqs"], d["rope"], d["append"], stream))
         if op != "append":
-            called(d, d["lib"].mossgpu_kv8_read(d["cache"], d["seqs"], d["read"], d["stream"]))
+            called(d, d["lib"].mossgpu_kv8_read(d["cache"], d["seqs"], d["read"], stream))
             return {"k": s["k_out"], "v": s["v_out"]}
         return {"codes": s["codes"].view(torch.float8_e4m3fn), "scales": s["scales"], "q": s["q_out"]}
     if op == "rope":
