@@ -26,6 +26,7 @@
 #include <math.h>
 #include <string.h>
 
+#include <initializer_list>
 #include <type_traits>
 
 #include "../../include/mossgpu.h"
@@ -471,6 +472,9 @@ extern "C" int mossgpu_token_logprobs(const mossgpu_logprob_args *args, void *cu
     if (!a.logprob && !a.entropy && a.top_k == 0) return op_errorf("%s: nothing is asked for", who);
     const size_t size = a.type == MOSSGPU_F32 ? 4 : 2;
     if (reinterpret_cast<uintptr_t>(a.logits) % size != 0) return op_errorf("%s: logits is not aligned to its type", who);
+    for (const void *p : {static_cast<const void *>(a.tokens), static_cast<const void *>(a.logprob), static_cast<const void *>(a.entropy),
+                          static_cast<const void *>(a.top_ids), static_cast<const void *>(a.top_logprobs)})
+        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return op_errorf("%s: a pointer is not aligned to its type", who);
     int dev = -1, *status = nullptr;
     if (op_device(&dev, &status, who) != 0) return 1;
     const cudaStream_t st = static_cast<cudaStream_t>(cuda_stream);

@@ -31,6 +31,16 @@ def test_head_counts_at_the_end_of_their_type(M):
         T.refused(M, M.lib().mossgpu_kv8_append(T.cache(M), T.seqs(M, rows=1), T.rope(M), a, None), "above 2^30")
 
 
+@pytest.mark.parametrize("name", ["tokens", "logprob", "entropy", "top_ids", "top_logprobs"])
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_misaligned_logprob_pointers(M, name, off):
+    # every pointer that the device would read or write 4 bytes at
+    import test_op_refusals as T
+    a = dict(logits=T.P, tokens=T.P, logprob=T.P, entropy=T.P, top_ids=T.P, top_logprobs=T.P, row_stride=100, rows=2, vocab=100, top_k=4,
+             temperature=1.0)
+    T.refused(M, M.lib().mossgpu_token_logprobs(M.LogprobArgs(**{**a, name: T.P + off}), None), "aligned to its type")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,t", [(8192, torch.float32), (65536, torch.bfloat16), (65536, torch.float16)])
 def test_rows_claimed_by_many_sequences(M, L, rows, t):
