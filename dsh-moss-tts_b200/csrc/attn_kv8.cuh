@@ -176,9 +176,9 @@ __device__ __forceinline__ void query_factors(float top, float scale, float &to,
 __device__ __forceinline__ float score_base(float m) { return m == -INFINITY ? 0.f : m; }
 // What earlier sums are multiplied by when the maximum goes from m0 to m and the V scales' exponent from E0 to E
 __device__ __forceinline__ float sums_factor(float m0, float m, float rf, float E0, float E) { return ex2(fmaf(m0 - score_base(m), rf, E0 - E)); }
-// Partial sums are kept relative to their maximum alone, which is stored in log2 (finite where there is any): sums
-// relative to `bias` - E times this
-__device__ __forceinline__ float part_factor(float E, int bias) { return pow2i(int(E) - bias); }
+// Partial sums are kept relative to their maximum, which is stored in log2 (finite where there is any), and 2^-20, so
+// that a million positions' values of any size add up: sums relative to `bias` - E times this
+__device__ __forceinline__ float part_factor(float E, int bias) { return pow2i(int(E) - bias - 20); }
 __device__ __forceinline__ float part_reference(float m, float rf) { return m == -INFINITY ? m : fmaxf(fminf(m * rf, 0.5f * FLT_MAX), -0.5f * FLT_MAX); }
 
 // The bits of a scale's size, 0 for infinity and NaN

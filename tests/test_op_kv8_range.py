@@ -208,3 +208,36 @@ def test_nan_only_where_it_is_seen(M, L, form, t, fmt, dim, half):
     clean, mass, top = exact(cache, q.double(), starts, slots, 0.125, mask)
     fine = ~want
     assert ((got - clean).abs() <= R.attend_tolerance(mass, top, clean, t))[fine].all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
+def test_sums_of_the_largest_values(M, L, form, t, fmt, dim):
+    # 2000 equal weights of values of about 2^120, whose sum is past the range of fp32
+    cache, q, starts, slots, new, group = setup(form, fmt, dim, t)
+    q.zero_()
+    cache.codes[:, 1] = 100 if fmt == R.INT8 else 0x6c  # 96 in e4m3
+    cache.scales[:, 1] = 2.0**114
+    value = 2.0**114 * (100 if fmt == R.INT8 else 96)
+    got = run(M, L, cache, q, starts, slots, 0.125)
+    assert ((got - value).abs() <= value * (2.0**-19 + (2.0**-11 + 2.0**-8 if t == BF16 else 0.0))).all()
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("t", [F32, BF16])
+@pytest.mark.parametrize("fmt,dim", [(R.INT8, 64), (R.E4M3, 128)])
+@pytest.mark.parametrize("k,v", [(2.0**100, 2.0**-87), (2.0**-100, 2.0**100)])
+def test_scales_at_the_ends_of_their_range(M, L, form, t, fmt, dim, k, v):
+    cache, q, starts, slots, new, group = setup(form, fmt, dim, t)
+    for s, slot in enumerate(slots):
+        n = CTX[s] + new
+        for half, size in ((0, k), (1, v)):
+            pos = torch.arange(n)
+            page = cache.table[slot].long()[pos // 16]
+            cache.scales[page, half, :, pos % 16] = torch.ldexp(0.5 + torch.rand(n, cache.kvh, generator=torch.Generator().manual_seed(half)) / 2,
+                                                                torch.tensor(float(torch.tensor(size).log2())))
+    q = (q.double() / k / 50).to(t)
+    want, mass, top = exact(cache, q.double(), starts, slots, 0.125)
+    got = run(M, L, cache, q, starts, slots, 0.125)
+    assert ((got - want).abs() <= tolerance(cache, q, want, mass, top, starts, slots, t, group)).all()
