@@ -96,13 +96,15 @@ def seen_scale(cache, starts, slots, mask=None):
     return top, count
 
 
-def tolerance(cache, q, want, mass, top, starts, slots, t, group, mask=None):
+def tolerance(form, cache, q, want, mass, top, starts, slots, t, group, mask=None):
     """attend_tolerance, and what a weight's fp16 parts lose below 2^-14 of their range: half a step of 2^-24 where the
     largest weight times the largest V scale lies in [2^13, 2^14), so 2^-38 of that scale, for every position and its
-    largest code, relative to a sum of weights of at least 1 (the largest)."""
+    largest code, relative to a sum of weights of at least 1 (the largest).  The form for many rows leaves bf16 outputs
+    2^6 of room above, so 2^-32."""
+    low = 2.0**-32 if form == "many" and t == BF16 else 2.0**-38
     sv, count = seen_scale(cache, starts, slots, mask)
     sv = sv.repeat_interleave(group, 1)
-    return R.attend_tolerance(mass, top, want, t) + (2.0**-38 * R.CODE_MAX[cache.fmt] * count * sv)[..., None]
+    return R.attend_tolerance(mass, top, want, t) + (low * R.CODE_MAX[cache.fmt] * count * sv)[..., None]
 
 
 @pytest.mark.parametrize("form", list(FORMS))
@@ -120,7 +122,7 @@ def test_queries_and_v_scales_of_any_size(M, L, form, t, fmt, dim, size):
     scale = float(torch.tensor(0.125 / size, dtype=torch.float32))
     want, mass, top = exact(cache, q.double(), starts, slots, scale)
     got = run(M, L, cache, q, starts, slots, scale)
-    assert ((got - want).abs() <= tolerance(cache, q, want, mass, top, starts, slots, t, group)).all()
+    assert ((got - want).abs() <= tolerance(form, cache, q, want, mass, top, starts, slots, t, group)).all()
 
 
 @pytest.mark.parametrize("form", list(FORMS))
@@ -160,7 +162,7 @@ def test_scores_of_any_size(M, L, form, t, fmt, dim, scale):
     v = cache.heads(slots[0], CTX[0], 1)[[5, 6, 700, 1989]].mean(0).repeat_interleave(group, 0)
     assert ((want[long_rows] - v).abs() <= 1e-12 * mass[long_rows]).all()
     got = run(M, L, cache, q, starts, slots, scale)
-    tol = tolerance(cache, q, want, mass, torch.zeros(q.shape[:2], dtype=torch.float64), starts, slots, t, group)
+    tol = tolerance(form, cache, q, want, mass, torch.zeros(q.shape[:2], dtype=torch.float64), starts, slots, t, group)
     assert ((got - want).abs() <= tol).all()
 
 
@@ -181,7 +183,7 @@ def test_hidden_v_scales_do_not_count(M, L, form, t, fmt, dim, causal):
         mask = torch.tensor([[1 << i | (1 << (i - 1) if i > 1 else 0)] for _ in CTX for i in range(new)], dtype=torch.int32)
     want, mass, top = exact(cache, q.double(), starts, slots, 0.125, mask)
     got = run(M, L, cache, q, starts, slots, 0.125, mask)
-    tol = tolerance(cache, q, want, mass, top, starts, slots, t, group, mask)
+    tol = tolerance(form, cache, q, want, mass, top, starts, slots, t, group, mask)
     rows = torch.tensor([t != F16 or r % new != hidden for r in range(starts[-1])])
     assert ((got - want).abs() <= tol)[rows].all()
 
@@ -240,4 +242,4 @@ def test_scales_at_the_ends_of_their_range(M, L, form, t, fmt, dim, k, v):
     q = (q.double() / k / 50).to(t)
     want, mass, top = exact(cache, q.double(), starts, slots, 0.125)
     got = run(M, L, cache, q, starts, slots, 0.125)
-    assert ((got - want).abs() <= tolerance(cache, q, want, mass, top, starts, slots, t, group)).all()
+    assert ((got - want).abs() <= tolerance(form, cache, q, want, mass, top, starts, slots, t, group)).all()
