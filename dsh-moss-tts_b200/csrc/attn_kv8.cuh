@@ -7,13 +7,13 @@
 // positions come in tiles of 32 (two pages).  All tiles of one head, in order, are cut into equal
 // runs, one run of one head per warp of the grid: however ragged the batch is, every warp has the
 // same work.  The heads of a run go to neighbouring warps, since a page's heads lie side by side (512
-// long sequences: 364 us against 372 with the runs of a head behind one another).  A warp that has a whole
+// long sequences: with the runs of a head behind one another 2% more time).  A warp that has a whole
 // unit writes its rows; a unit cut between warps leaves partial sums in the workspace, which k_attn_kv8_join (a
 // dependent launch) merges in a fixed order, so that a result does not depend on timing.
 //
 // A tile.  K, V and their scales of the pages (each contiguous) are copied to a stage of the warp's own
-// ring in shared memory, 16 bytes a lane (339 us for those sequences against 362 with bulk copies of 1 KB,
-// which are issued one lane after the other).  No barrier but the warp's own.  S = q K^T
+// ring in shared memory, 16 bytes a lane (with bulk copies of 1 KB, which are issued one lane after the
+// other, those sequences take 7% more).  No barrier but the warp's own.  S = q K^T
 // and o += w V are mma.sync m16n8k16 products in fp16, in which every 8-bit code is exact.  Which
 // element of the head dimension is the k-th of a product, and which position is the n-th, is free as
 // long as both operands agree.  Here a lane takes 16 consecutive codes of a K row, the same columns of
@@ -30,9 +30,9 @@
 // tensor cores truncate when they accumulate, such products start from zero every tile and are added
 // in fp32.  Statistics, sums and partials are fp32.
 //
-// Measured on one B200: 512 sequences of 256-4096 positions, 12 heads of 64, int8: 300 us (6.1 TB/s, 93%
-// of the measured copy rate) in short bursts, 323-343 us (81-86%) when repeated for seconds, as the card then
-// lowers its clocks: about 450 instructions a tile of 32 positions keep the schedulers 62% busy.
+// Measured on one B200: 512 sequences of 256-4096 positions, 12 heads of 64, int8: 301 us (6.0 TB/s, 92%
+// of the measured copy rate) in bursts of 20 calls, 318-345 us (81-87%, by card) when repeated for seconds, as the
+// card then lowers its clocks: about 455 instructions a tile of 32 positions keep the schedulers 62% busy.
 #pragma once
 
 #include <float.h>
@@ -797,7 +797,7 @@ __global__ void __launch_bounds__(Ak8Shape<D>::kWarps * 32, 1) k_attn_kv8(const 
 }
 
 // Units of more rows.  A CTA's four warps take 8 or 16 of them each; a tile is read once for all of
-// them (64 rows of bf16 over an e4m3 cache of heads of 128: 175 TFLOP/s; three warps a scheduler wait for
+// them (64 rows of bf16 over an e4m3 cache of heads of 128: 171 TFLOP/s; three warps a scheduler wait for
 // one another's shared-memory reads, 56% of that pipe, and products, 27% of theirs), and its codes are converted to fp16 once, each thread its share, a tile ahead of its use (the
 // conversions are as many instructions as the rest of a tile's work).  The warps take their fragments
 // from the converted tile with ldmatrix; its 16-byte chunks are stored at chunk ^ (row % 8).  A run

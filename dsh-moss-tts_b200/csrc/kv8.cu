@@ -133,8 +133,9 @@ AttnForm attn_rows(int64_t rows_per_unit, bool direct) {
     constexpr int kRows = Rows<D, MODE>::kRows;
     if (direct) return {k_attn_kv8<D, FORMAT, MODE, true>, S::kWarps, 1, S::kRing, kRows, 0};
     // A warp a unit reads and converts a tile again for every 8 or 16 rows, a CTA once for 32 or 64, but takes as
-    // long for few of them.  48 sequences of 700-8000 positions, 8 kv heads of 128, e4m3 (us when repeated for a
-    // second; warp, CTA): 20 rows 208, 253; 32 rows 219, 258; 48 rows 319, 294; 64 rows 404, 318; 96 rows 606, 554.
+    // long for few of them.  48 sequences of 700-8000 positions, 8 kv heads of 128, e4m3, bf16 (us when repeated for a
+    // second; warp, CTA): 20 rows 212, 252; 32 rows 224, 258; 48 rows 324, 296; 64 rows 430, 320; 96 rows 626, 555.
+    // The other types, sizes and formats go by the same count of rows a product, unmeasured.
     if (rows_per_unit <= 2 * kRows) return {k_attn_kv8<D, FORMAT, MODE, false>, S::kWarps, 1, S::kRing, kRows, kNumSMs * S::kWarps};
     return {k_attn_kv8_block<D, FORMAT, MODE>, B::kWarps, B::kCtas, B::kRing, B::kWarps * kRows, kNumSMs * B::kCtas};
 }
@@ -142,12 +143,13 @@ AttnForm attn_rows(int64_t rows_per_unit, bool direct) {
 template <int D, int FORMAT>
 AttnForm attn_form(int type, int64_t rows_per_unit, int64_t rows, int n_seqs, int kv_heads, int pages) {
     // A CTA a unit (one launch) where that is few rounds of CTAs and no warp gets more than 8 tiles of 32
-    // positions.  Us, one launch against two, 12 heads of 64: one stream of 300 positions 6.9, 10.9; 8 x 1000 8.9,
-    // 16.8; 32 x 1000 (480 units) 21.1, 24.1; but 32 x 100-3000 29.1, 27.3, and one of 4000 17.0, 14.3.
+    // positions, which is known by the width of the table alone.  Us, one launch against two, 12 heads of 64: one stream
+    // of 300 positions 7.0, 10.8; 8 x 1000 8.3, 16.5; 32 x 1000 (480 units) 20.6, 24.6; but 32 x 100-3000 27.1, 26.8,
+    // and one of 4000 16.5, 14.4.
     const auto direct = [&](int tile_rows, int warps) { return (rows / tile_rows + n_seqs) * kv_heads <= 4 * kNumSMs && pages <= 2 * 8 * warps; };
-    // The form for 4 rows takes 8 in two units.  Streams of 256-4096 positions, 12 kv heads of 64, int8 (us when
-    // repeated for a second; this form, the next): one row of 512 streams 335, 380; 4 rows of 128 streams 96, 113; 8
-    // rows 177, 114.
+    // The form for 4 rows takes 8 in two units.  Streams of 256-4096 positions, 12 kv heads of 64, int8, fp32 (us when
+    // repeated for a second; this form, the next, on one card): one row of 512 streams 345, 386; 4 rows of 128 streams
+    // 98, 109; 8 rows 180, 114.
     if (rows_per_unit <= 4) {
         using S = Ak8Few<D>;
         if (direct(4, S::kWarps)) return {k_attn_kv8_few<D, FORMAT, true>, S::kWarps, 1, S::kRing, 4, 0};

@@ -15,8 +15,8 @@
 // counting.  Rows where that does not work -- NaN, or more ties than the buffer holds -- find the
 // exact k-th (logit, id) by bisection instead, over the row as it lies in the cache.
 //
-// Measured on one B200: 8192 rows of 1024 (fp32, k = 8) 16.4 us, 2.1 TB/s: about 1000 instructions a row, a
-// warp each; 160 rows of 128001 (bf16, k = 20) 30.7 us: 148 rows fit at once, and the selection is a third.
+// Measured on one B200: 8192 rows of 1024 (fp32, k = 8) 16.3 us, 2.1 TB/s: about 1000 instructions a row, a
+// warp each; 160 rows of 128001 (bf16, k = 20) 30.7 us: 148 rows fit at once, and the selection is more than a third.
 #include <cooperative_groups.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

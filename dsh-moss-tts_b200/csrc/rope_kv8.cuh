@@ -206,7 +206,8 @@ __device__ __forceinline__ LaneRope<LAYOUT> lane_rope(const mossgpu_rope &r, int
     }
     return t;
 }
-// x[0..3] and x[4..7]: the two chunks.  Elements that do not turn stay as they are, whatever their bits.
+// x[0..3] and x[4..7]: the two chunks.  Elements that do not turn keep their values (the payload of a
+// 16-bit NaN may change on its way through fp32).
 // All lanes of the warp call the kAny form; `stage`: 256 floats of this warp, lph lanes a head.
 template <int LAYOUT>
 __device__ __forceinline__ void rope_turn(float (&x)[8], const LaneRope<LAYOUT> &t, const mossgpu_rope &r, float *stage, int lph) {

@@ -285,9 +285,11 @@ int mossgpu_attention_decode_paged_noalloc(const float *q, const void *kv_layer,
  * call of an op on a device loads its kernels: make that one outside a capture).  The descriptors
  * are host structs, read before the call returns.  Errors: non-zero return, message from
  * mossgpu_op_last_error() (per thread); a refused call enqueues nothing.  Values that only the
- * device sees (row bounds, slots, positions, page ids, tokens) are checked there: what is out of
- * range is skipped and recorded for mossgpu_op_device_status: 9 = a slot or position outside the
- * page table, 10 = a page id outside the pool, 11 = a token id >= vocab.
+ * device sees (row bounds, slots, positions, page ids, tokens) are checked there.  Row bounds are cut
+ * to the rows, without a record; what else is out of range is skipped and recorded for
+ * mossgpu_op_device_status: 9 = a slot or position outside the page table, or (attention) row bounds
+ * that do not ascend and claim more rows than can be counted, which leaves all rows as they are;
+ * 10 = a page id outside the pool, 11 = a token id >= vocab.
  *
  * Element types of activations: */
 enum { MOSSGPU_F32 = 0, MOSSGPU_F16 = 1, MOSSGPU_BF16 = 2 };
@@ -299,7 +301,7 @@ enum { MOSSGPU_F32 = 0, MOSSGPU_F16 = 1, MOSSGPU_BF16 = 2 };
 /* Rotary positions.  Pair i < rotary_dim / 2 of a head turns by pos * f_i:
  *   y_a = magnitude (x_a cos - x_b sin),  y_b = magnitude (x_b cos + x_a sin)
  * with (a, b) = (2i, 2i + 1) when interleaved, (i, i + rotary_dim / 2) otherwise; elements from
- * rotary_dim on are copied.  The angle is held in whole 2^-64 turns: `steps` is
+ * rotary_dim on are copied (a NaN of 16 bits as a NaN, not bit by bit).  The angle is held in whole 2^-64 turns: `steps` is
  * round(f_i / (2 pi) 2^64) modulo 2^64, so that pos * steps, taken modulo 2^64, is the reduced
  * angle at any position, without the loss that a product of floats has at far ones. */
 typedef struct {
@@ -327,7 +329,7 @@ int mossgpu_rope_steps(int rotary_dim, double base, const mossgpu_rope_scaling *
 
 /* out = x rotated (or turned back, which is also the gradient of the rotation): x, out
  * [rows][heads][head_dim], head_dim a multiple of 8 up to 256.  out may be x itself with the same
- * strides, or must not overlap it. */
+ * strides, or must not overlap it.  At most 2^30 heads. */
 typedef struct {
     const void *x;
     void *out;
@@ -403,6 +405,10 @@ int mossgpu_kv8_read(const mossgpu_kv8_cache *cache, const mossgpu_seq_batch *se
  * the decode step of a single token.  New rows past 32 * mask_words are not seen.  q_heads is a
  * multiple of kv_heads; head h reads kv head h / (q_heads / kv_heads).
  *   out = sum_j p_j V_j,  p = softmax_j(scale q.K_j);  a row that sees nothing gives zeros
+ * Queries, scale and scores may have any finite size.  K scales up to 2^100 and V scales of 2^-87 to
+ * 2^100 keep the products' bits (22; the weights of bf16 outputs 11), and so does a position whose V
+ * scale is within 2^20 of the largest that its row sees: below that its share is right to 2^-38 (bf16
+ * outputs 2^-32) of the largest.  What a row does not see has no influence on it.
  * The workspace (any contents, 16-byte aligned, at least mossgpu_attention_kv8_workspace_bytes)
  * belongs to the call until it has run: two calls that may overlap need two. */
 typedef struct {
