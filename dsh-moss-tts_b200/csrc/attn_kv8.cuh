@@ -24,8 +24,9 @@
 // Precision.  A query row is scaled by a power of two to [128, 256) and rounded to fp16, exact for
 // bf16 and fp16 inputs.  Weights are w = 2^(rf (s - m) + 140 - E) sv, s the scores without the row's factor rf, m
 // their running maximum and E the exponent of the largest V scale that the row has seen: w < 2^14 fits fp16
-// whatever the scales are, and, since the difference comes before the factor, however large the scores are.  For bf16 outputs w is rounded to fp16 (2^-11 against the output's
-// 2^-8), 16 rows a product.  For fp32 and fp16 outputs q and w are split into an upper and a lower
+// whatever the scales are, and, since the difference comes before the factor, however large the scores are.
+// For bf16 outputs w is rounded to fp16 (2^-11 against the output's 2^-8), 16 rows a product.  For fp32 and
+// fp16 outputs q and w are split into an upper and a lower
 // fp16 part (22 bits) that occupy rows g and g + 8 of the same product, 8 rows a product; since the
 // tensor cores truncate when they accumulate, such products start from zero every tile and are added
 // in fp32.  Statistics, sums and partials are fp32.
